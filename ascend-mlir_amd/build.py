@@ -44,6 +44,9 @@ KERNEL_SOURCES = [
     ("kernels/matmul.hip", []),
     ("kernels/matmul_dma.hip", []),
     ("kernels/matmul_layouts.hip", []),
+    ("kernels/mxfp4_quantize.hip", []),
+    ("kernels/mxfp4_matmul.hip", []),
+    ("kernels/norm_gate.hip", []),
     ("kernels/region.hip", STRICT),
     ("target/region_program.cpp", []),
     ("target/hip_emitter.cpp", []),

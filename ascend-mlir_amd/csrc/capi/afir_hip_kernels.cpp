@@ -563,6 +563,70 @@ uint32_t afir_hip_launch_matmul_add_leakyrelu(uint32_t block_dim, void *stream, 
 }
 
 namespace {
+float field_as_float(int64_t field) {
+  const uint32_t bits = (uint32_t)((uint64_t)field & 0xffffffffu);
+  float v;
+  std::memcpy(&v, &bits, 4);
+  return v;
+}
+}  // namespace
+
+uint32_t afir_hip_launch_mxfp4_quantize(uint32_t block_dim, void *stream, void *x, void *codes, void *scales,
+                                        void *values, void * /*workspace*/, void *tiling) {
+  int64_t f[5];
+  if (!read_fields(tiling, 5, f)) return fail(AFIR_HIP_E_INVALID, "mxfp4_quantize: null tiling");
+  if (f[3] != 0 && f[3] != 1) return fail(AFIR_HIP_E_INVALID, "mxfp4_quantize: axis must be 0 or 1");
+  const bool columns = f[3] == 0;
+  return finish(afir::launch_mxfp4_quantize(x, f[2], codes, scales, values, columns ? f[1] : f[0],
+                                            columns ? f[0] : f[1], columns, (int)f[4], block_dim,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+uint32_t afir_hip_launch_mxfp4_matmul_add_leakyrelu(uint32_t block_dim, void *stream, void *a, void *a_scales, void *b,
+                                                    void *b_scales, void *bias, void *out, void *workspace,
+                                                    void *tiling) {
+  int64_t f[5];
+  if (!read_fields(tiling, 5, f)) return fail(AFIR_HIP_E_INVALID, "mxfp4_matmul_add_leakyrelu: null tiling");
+  return finish(afir::launch_mxfp4_matmul(a, a_scales, b, b_scales, bias, out, f[0], f[1], f[2], field_as_float(f[3]),
+                                          (int)f[4], workspace, block_dim, static_cast<hipStream_t>(stream)));
+}
+
+size_t afir_hip_mxfp4_matmul_workspace_bytes(const void *tiling) {
+  int64_t f[5];
+  return read_fields(tiling, 5, f) ? afir::mxfp4_matmul_workspace(f[0], f[1], f[2]) : 0;
+}
+
+uint32_t afir_hip_launch_norm_gate_residual(uint32_t block_dim, void *stream, void *x, void *f, void *post_weight,
+                                            void *gate, void *pre_weight, void *y, void *h, void * /*workspace*/,
+                                            void *tiling) {
+  int64_t t[11];
+  if (!read_fields(tiling, 11, t)) return fail(AFIR_HIP_E_INVALID, "norm_gate_residual: null tiling");
+  afir::NormGateArgs p{x, f, post_weight, gate, pre_weight, y, h, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7],
+                       field_as_float(t[8]), field_as_float(t[9]), 0.f};
+  return finish(afir::launch_norm_gate_residual(p, (int)t[10], block_dim, static_cast<hipStream_t>(stream)));
+}
+
+uint32_t afir_hip_launch_norm_gate_residual_backward(uint32_t block_dim, void *stream, void *dy, void *dh, void *y, void *f,
+                                                     void *post_weight, void *gate, void *pre_weight, void *dx, void *df,
+                                                     void *dpost_weight, void *dgate, void *dpre_weight, void *workspace,
+                                                     void *tiling) {
+  int64_t t[13];
+  if (!read_fields(tiling, 13, t)) return fail(AFIR_HIP_E_INVALID, "norm_gate_residual_backward: null tiling");
+  afir::NormGateGradArgs p{dy, dh, y, f, post_weight, gate, pre_weight, dx, df, dpost_weight, dgate, dpre_weight,
+                           static_cast<float *>(workspace), t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9],
+                           field_as_float(t[10]), field_as_float(t[11]), 0.f};
+  return finish(afir::launch_norm_gate_residual_backward(p, (int)t[12], block_dim, static_cast<hipStream_t>(stream)));
+}
+
+size_t afir_hip_norm_gate_residual_backward_workspace_bytes(const void *tiling) {
+  int64_t t[13];
+  if (!read_fields(tiling, 13, t)) return 0;
+  const size_t with = afir::norm_gate_backward_workspace(t[0], t[1], t[2], true, (int)t[12]);
+  const size_t without = afir::norm_gate_backward_workspace(t[0], t[1], t[2], false, (int)t[12]);
+  return with > without ? with : without;
+}
+
+namespace {
 uint32_t register_region(const char *program_text, size_t program_len, uint64_t *handle, bool generic);
 }
 

@@ -1,0 +1,561 @@
+// The norms before and after a residual block, fused with the gate and the residual sum:
+//
+//   y = s * x + gate * (f * rstd(f)) * post_weight        rstd(v) = 1 / sqrt(mean(v^2) + eps)
+//   h = y * rstd(y) * pre_weight                           (y unrounded)
+//
+// f is what the block gave, h what the next one takes, x and y the residual stream.  Without f, y
+// is x itself (the norm ahead of the first block); without pre_weight there is no h.  A gate row
+// serves rows_per_gate rows: 1 for a gate per element, a sequence's length for a modulated block, M
+// for one learned row.
+//
+// Memory-bound: forward reads x and f and writes y and h, backward reads the gradients of y and h,
+// y and f, and writes the gradients of x and f.  A row stays in registers from its load to its
+// store: the two row sums (forward) and the two rounds of row sums (backward) are the only
+// exchange between lanes.  All arithmetic is float32, each result rounded once as it is stored.
+#include "kernels.h"
+#include "mxfp4.h"
+
+namespace afir {
+
+namespace {
+
+// What a lane holds of a row: ITEMS 16-byte pieces, lanes adjacent.
+template <int KIND, int ITEMS>
+struct Piece {
+  uint32_t w[ITEMS][4];
+};
+
+// Row pieces of a lane; numbers past the row's end are zeros and add nothing to any sum.  (A
+// 16-byte access needs the alignment of an element only, see mxfp4.h.)
+template <int KIND, int LANES, int ITEMS>
+__device__ __forceinline__ void load_row(const void *base, int64_t offset, int lane, int64_t n, Piece<KIND, ITEMS> &p) {
+  constexpr int V = Elem<KIND>::kPer16;
+  typedef typename Elem<KIND>::type T;
+  const T *row = static_cast<const T *>(base) + offset;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t e = (int64_t)(lane + i * LANES) * V;
+    p.w[i][0] = p.w[i][1] = p.w[i][2] = p.w[i][3] = 0;
+    if (e + V <= n) {
+      const u32x4 v = *reinterpret_cast<const u32x4_u *>(row + e);
+      p.w[i][0] = v.x; p.w[i][1] = v.y; p.w[i][2] = v.z; p.w[i][3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V - 1; ++j)
+        if (e + j < n) {
+          if constexpr (V == 8) p.w[i][j / 2] |= (uint32_t)row[e + j] << (16 * (j & 1));
+          else p.w[i][j] = __float_as_uint(row[e + j]);
+        }
+    }
+  }
+}
+template <int KIND, int LANES>
+__device__ __forceinline__ void store_item(void *base, int64_t offset, int64_t e, int64_t n,
+                                           const float (&v)[Elem<KIND>::kPer16]) {
+  constexpr int V = Elem<KIND>::kPer16;
+  typedef typename Elem<KIND>::type T;
+  T *row = static_cast<T *>(base) + offset;
+  if (e + V <= n) {
+    uint32_t w[4];
+    Elem<KIND>::pack(v, w);
+    *reinterpret_cast<u32x4_u *>(row + e) = u32x4{w[0], w[1], w[2], w[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < V - 1; ++j)
+      if (e + j < n) Elem<KIND>::store(row, e + j, v[j]);
+  }
+}
+
+// Sums over the WAVES wavefronts of a row, in a fixed order.  Calls alternate between two slots
+// (`turn`), so the barrier of a call also separates the reads of the call before it from the writes
+// of the call after it, which go to the same slot.
+template <int WAVES, int COUNT>
+__device__ __forceinline__ void row_sums(float (&v)[COUNT], float *lds, int &turn, int wave) {
+#pragma unroll
+  for (int c = 0; c < COUNT; ++c) v[c] = wave_sum(v[c]);
+  if constexpr (WAVES > 1) {
+    float *part = lds + turn * (WAVES * 4);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int c = 0; c < COUNT; ++c) part[wave * 4 + c] = v[c];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += part[w * 4 + c];
+      v[c] = s;
+    }
+  }
+}
+
+__device__ __forceinline__ float rstd_of(float sum_of_squares, float inv_n, float eps) {
+  return 1.0f / sqrtf(sum_of_squares * inv_n + eps);
+}
+
+constexpr int threads_of(int waves) { return waves == 1 ? 256 : waves * 64; }   // single-wave rows: four to a workgroup
+
+template <int KIND, int WAVES, int ITEMS>
+__global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateArgs p) {
+  constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64, kRowsHere = threads_of(WAVES) / kLanes;
+  __shared__ float lds[2 * WAVES * 4];
+  const int lane = threadIdx.x % kLanes, wave = lane >> 6;
+  const int64_t n = p.n;
+  Piece<KIND, ITEMS> post, pre;
+  if (p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
+  if (p.h) load_row<KIND, kLanes, ITEMS>(p.pre_weight, 0, lane, n, pre);
+  const int64_t stride = (int64_t)gridDim.x * kRowsHere;
+  int64_t row = (int64_t)blockIdx.x * kRowsHere + threadIdx.x / kLanes;
+  int turn = 0;
+  Piece<KIND, ITEMS> x, f, gate;
+  auto fetch = [&](int64_t r) {
+    load_row<KIND, kLanes, ITEMS>(p.x, r * p.ld_x, lane, n, x);
+    if (p.f) {
+      load_row<KIND, kLanes, ITEMS>(p.f, r * p.ld_f, lane, n, f);
+      if (p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+    }
+  };
+  if (row < p.m) fetch(row);
+  for (; row < p.m; row += stride) {
+    float y[ITEMS][V];
+    if (p.f) {
+      float sum[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float v[V];
+        Elem<KIND>::unpack(f.w[i], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[0] += v[j] * v[j];
+      }
+      row_sums<WAVES>(sum, lds, turn, wave);
+      const float rf = rstd_of(sum[0], p.inv_n, p.eps);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float vx[V], vf[V], vg[V], vw[V];
+        Elem<KIND>::unpack(x.w[i], vx);
+        Elem<KIND>::unpack(f.w[i], vf);
+        Elem<KIND>::unpack(post.w[i], vw);
+        if (p.gate) Elem<KIND>::unpack(gate.w[i], vg);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float b = vf[j] * rf * vw[j];
+          y[i][j] = p.residual_scale * vx[j] + (p.gate ? vg[j] * b : b);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) Elem<KIND>::unpack(x.w[i], y[i]);
+    }
+    if (row + stride < p.m) fetch(row + stride);
+    if (p.y)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        store_item<KIND, kLanes>(p.y, row * p.ld_y, (int64_t)(lane + i * kLanes) * V, n, y[i]);
+    if (p.h) {
+      float sum[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[0] += y[i][j] * y[i][j];
+      row_sums<WAVES>(sum, lds, turn, wave);
+      const float ry = rstd_of(sum[0], p.inv_n, p.eps);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float vw[V], o[V];
+        Elem<KIND>::unpack(pre.w[i], vw);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = y[i][j] * ry * vw[j];
+        store_item<KIND, kLanes>(p.h, row * p.ld_h, (int64_t)(lane + i * kLanes) * V, n, o);
+      }
+    }
+  }
+}
+
+template <int KIND, int WAVES, int ITEMS>
+LaunchStatus forward_launch(const NormGateArgs &p, uint32_t block_dim, hipStream_t stream) {
+  constexpr int kRowsHere = threads_of(WAVES) / (WAVES * 64);
+  int64_t blocks = (p.m + kRowsHere - 1) / kRowsHere;
+  const int64_t most = (int64_t)device_cus() * 8;
+  if (blocks > most) blocks = most;
+  if (block_dim) blocks = block_dim;
+  AFIR_LAUNCH("norm_gate_forward", (norm_gate_forward<KIND, WAVES, ITEMS>), dim3((unsigned)blocks),
+              dim3(threads_of(WAVES)), 0, stream, p);
+  return after_launch();
+}
+
+template <int KIND>
+LaunchStatus forward(const NormGateArgs &p, uint32_t block_dim, hipStream_t stream) {
+  const int64_t pieces = (p.n + Elem<KIND>::kPer16 - 1) / Elem<KIND>::kPer16;
+  if (pieces <= 64) return forward_launch<KIND, 1, 1>(p, block_dim, stream);
+  if (pieces <= 128) return forward_launch<KIND, 1, 2>(p, block_dim, stream);
+  if (pieces <= 256) return forward_launch<KIND, 4, 1>(p, block_dim, stream);
+  if (pieces <= 512) return forward_launch<KIND, 4, 2>(p, block_dim, stream);
+  if (pieces <= 1024) return forward_launch<KIND, 4, 4>(p, block_dim, stream);
+  if constexpr (kNormMaxColumns / Elem<KIND>::kPer16 > 2048)
+    if (pieces > 2048) return forward_launch<KIND, 16, 4>(p, block_dim, stream);
+  return forward_launch<KIND, 16, 2>(p, block_dim, stream);
+}
+
+// ---- backward ----
+//
+// With yn = y rstd(y), fn = f rstd(f) and a = dh * pre_weight:
+//   t  = dy + rstd(y) (a - yn mean(a yn))            the gradient of the unscaled sum
+//   dx = s t          b = t gate post_weight
+//   df = rstd(f) (b - fn mean(b fn))
+//   dpost_weight = sum over rows of t gate fn         dpre_weight = sum over rows of dh yn
+//   dgate = post_weight * sum over the gate row's rows of t fn
+// mean(a yn) and both rstd need one round of row sums, mean(b fn) a second one; nothing is kept
+// from the forward pass but y.
+//
+// The column sums: a workgroup walks a stretch of rows and keeps its share of a row's columns in
+// registers, then writes one row of float32 partial sums, which a second kernel adds in a fixed
+// order.  A stretch never straddles two gate rows unless it covers each of them whole, so either
+// the gate is one row throughout (kOneGate: the partial sum is that of t fn, which serves dgate
+// and, weighted with the gate, dpost_weight), or dgate's rows are finished within the workgroup.
+struct Stretches {       // stretch i: rows from (i / per_span) * span + (i % per_span) * rows
+  int64_t span;          // rows of one gate row, or of several whole ones
+  int64_t per_span, rows, count;
+  bool one_gate;
+};
+
+inline Stretches plan_stretches(int64_t m, int64_t rows_per_gate, bool gate, int64_t workgroups) {
+  Stretches s;
+  int64_t rows = (m + workgroups - 1) / workgroups;
+  const int64_t per_gate = gate && rows_per_gate < m ? rows_per_gate : m;
+  if (gate && per_gate <= rows) {
+    s.one_gate = per_gate == m;
+    s.rows = s.span = rows / per_gate * per_gate;
+    s.per_span = 1;
+  } else {
+    s.one_gate = true;
+    s.span = per_gate;
+    s.per_span = (per_gate + rows - 1) / rows;
+    s.rows = (per_gate + s.per_span - 1) / s.per_span;
+  }
+  s.count = (m + s.span - 1) / s.span * s.per_span;
+  return s;
+}
+
+template <int KIND, int WAVES, int ITEMS, bool kOneGate>
+__global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArgs p, Stretches s) {
+  constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64;
+  __shared__ float lds[2 * WAVES * 4];
+  const int lane = threadIdx.x, wave = lane >> 6;
+  const int64_t n = p.n;
+  Piece<KIND, ITEMS> post, pre;
+  if (p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
+  if (p.dh) load_row<KIND, kLanes, ITEMS>(p.pre_weight, 0, lane, n, pre);
+  int turn = 0;
+  for (int64_t stretch = blockIdx.x; stretch < s.count; stretch += gridDim.x) {
+    const int64_t first = stretch / s.per_span * s.span, r0 = first + stretch % s.per_span * s.rows;
+    int64_t r1 = r0 + s.rows < first + s.span ? r0 + s.rows : first + s.span;
+    r1 = r1 < p.m ? r1 : p.m;
+    float acc_post[ITEMS][V], acc_pre[ITEMS][V], acc_gate[kOneGate ? 1 : ITEMS][V];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        acc_post[i][j] = acc_pre[i][j] = 0.f;
+        if constexpr (!kOneGate) acc_gate[i][j] = 0.f;
+      }
+    Piece<KIND, ITEMS> dy, dh, y, f, gate;
+    auto fetch = [&](int64_t r) {
+      if (p.dy) load_row<KIND, kLanes, ITEMS>(p.dy, r * p.ld_dy, lane, n, dy);
+      if (p.dh) {
+        load_row<KIND, kLanes, ITEMS>(p.dh, r * p.ld_dh, lane, n, dh);
+        load_row<KIND, kLanes, ITEMS>(p.y, r * p.ld_y, lane, n, y);
+      }
+      if (p.f) {
+        load_row<KIND, kLanes, ITEMS>(p.f, r * p.ld_f, lane, n, f);
+        if (!kOneGate && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      }
+    };
+    if (r0 < r1) {
+      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r0 / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      fetch(r0);
+    }
+    for (int64_t row = r0; row < r1; ++row) {
+      float sums[3] = {0.f, 0.f, 0.f};   // y^2, dh pre y, f^2
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        if (p.dh) {
+          float vy[V], vd[V], vw[V];
+          Elem<KIND>::unpack(y.w[i], vy);
+          Elem<KIND>::unpack(dh.w[i], vd);
+          Elem<KIND>::unpack(pre.w[i], vw);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            sums[0] += vy[j] * vy[j];
+            sums[1] += vd[j] * vw[j] * vy[j];
+          }
+        }
+        if (p.f) {
+          float vf[V];
+          Elem<KIND>::unpack(f.w[i], vf);
+#pragma unroll
+          for (int j = 0; j < V; ++j) sums[2] += vf[j] * vf[j];
+        }
+      }
+      row_sums<WAVES>(sums, lds, turn, wave);
+      const float ry = rstd_of(sums[0], p.inv_n, p.eps), rf = rstd_of(sums[2], p.inv_n, p.eps);
+      const float my = ry * sums[1] * p.inv_n;   // mean(a yn)
+      float t[ITEMS][V], vf[ITEMS][V], vg[ITEMS][V];
+      float dot[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        if (p.dy) Elem<KIND>::unpack(dy.w[i], t[i]);
+        else
+#pragma unroll
+          for (int j = 0; j < V; ++j) t[i][j] = 0.f;
+        if (p.dh) {
+          float vy[V], vd[V], vw[V];
+          Elem<KIND>::unpack(y.w[i], vy);
+          Elem<KIND>::unpack(dh.w[i], vd);
+          Elem<KIND>::unpack(pre.w[i], vw);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float yn = vy[j] * ry;
+            t[i][j] += ry * (vd[j] * vw[j] - yn * my);
+            acc_pre[i][j] += vd[j] * yn;
+          }
+        }
+        if (p.f) {
+          float vw[V];
+          Elem<KIND>::unpack(f.w[i], vf[i]);
+          Elem<KIND>::unpack(post.w[i], vw);
+          if (p.gate) Elem<KIND>::unpack(gate.w[i], vg[i]);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float gt = p.gate ? vg[i][j] * t[i][j] : t[i][j];
+            const float fn = vf[i][j] * rf;
+            dot[0] += gt * vw[j] * fn;
+            if constexpr (kOneGate) {
+              acc_post[i][j] += t[i][j] * fn;
+            } else {
+              acc_post[i][j] += gt * fn;
+              acc_gate[i][j] += t[i][j] * fn;
+            }
+          }
+        }
+      }
+      if (row + 1 < r1) fetch(row + 1);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = p.residual_scale * t[i][j];
+        store_item<KIND, kLanes>(p.dx, row * p.ld_dx, (int64_t)(lane + i * kLanes) * V, n, o);
+      }
+      if (p.f) {
+        row_sums<WAVES>(dot, lds, turn, wave);
+        const float mf = dot[0] * p.inv_n;   // mean(b fn)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          float o[V], vw[V];
+          Elem<KIND>::unpack(post.w[i], vw);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float b = (p.gate ? vg[i][j] * t[i][j] : t[i][j]) * vw[j];
+            o[j] = rf * (b - vf[i][j] * rf * mf);
+          }
+          store_item<KIND, kLanes>(p.df, row * p.ld_df, (int64_t)(lane + i * kLanes) * V, n, o);
+        }
+        if constexpr (!kOneGate) {
+          if ((row + 1) % p.rows_per_gate == 0 || row + 1 == p.m) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+              float o[V], vw[V];
+              Elem<KIND>::unpack(post.w[i], vw);
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                o[j] = acc_gate[i][j] * vw[j];
+                acc_gate[i][j] = 0.f;
+              }
+              store_item<KIND, kLanes>(p.dgate, row / p.rows_per_gate * n, (int64_t)(lane + i * kLanes) * V, n, o);
+            }
+          }
+        }
+      }
+    }
+    float *const part_post = p.partial + stretch * n, *const part_pre = p.partial + (s.count + stretch) * n;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int64_t e = (int64_t)(lane + i * kLanes) * V + j;
+        if (e < n) {
+          if (p.f) part_post[e] = acc_post[i][j];
+          if (p.dh) part_pre[e] = acc_pre[i][j];
+        }
+      }
+  }
+}
+
+// Adds the partial rows: blockIdx.y 0 gives dpre_weight, 1 dpost_weight, 2 + g gate row g (kOneGate
+// launches with a gate).  64 columns per workgroup, sixteen wavefronts share the rows.
+constexpr int kJoinWaves = 16;
+template <int KIND>
+__global__ __launch_bounds__(kJoinWaves * 64) void norm_gate_join(NormGateGradArgs p, Stretches s, int64_t column_tiles) {
+  __shared__ float lds[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int what = blockIdx.y;
+  if ((what == 0 && !p.dh) || (what == 1 && !p.f)) return;
+  const float *const part = p.partial + (what == 0 ? s.count * p.n : 0);
+  const int64_t first = what < 2 ? 0 : (what - 2) * s.per_span, last = what < 2 ? s.count : first + s.per_span;
+  const bool weighted = what == 1 && s.one_gate && p.gate;
+  for (int64_t tile = blockIdx.x; tile < column_tiles; tile += gridDim.x) {
+    const int64_t e = tile * 64 + lane;
+    float v = 0.f;
+    if (e < p.n) {
+      if (weighted) {
+        for (int64_t r = first + wave; r < last; r += kJoinWaves)
+          v += part[r * p.n + e] * Elem<KIND>::load(p.gate, r / s.per_span * p.ld_gate + e);
+      } else {
+#pragma unroll 4
+        for (int64_t r = first + wave; r < last; r += kJoinWaves) v += part[r * p.n + e];
+      }
+    }
+    lds[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && e < p.n) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWaves; ++w) sum += lds[w][lane];
+      if (what == 0) Elem<KIND>::store(p.dpre_weight, e, sum);
+      else if (what == 1) Elem<KIND>::store(p.dpost_weight, e, sum);
+      else Elem<KIND>::store(p.dgate, (what - 2) * p.n + e, sum * Elem<KIND>::load(p.post_weight, e));
+    }
+    __syncthreads();
+  }
+}
+
+// Wavefronts a row of the backward pass is spread over, and 16-byte pieces per lane.
+struct RowShape {
+  int waves, items;
+};
+inline RowShape backward_shape(int64_t n, int elem_kind) {
+  const int64_t pieces = elem_kind == kElemF32 ? (n + 3) / 4 : (n + 7) / 8;
+  if (pieces <= 64) return {1, 1};
+  if (pieces <= 128) return {1, 2};
+  if (pieces <= 256) return {4, 1};
+  if (pieces <= 512) return {4, 2};
+  if (pieces <= 1024) return {4, 4};
+  if (pieces <= 2048) return {8, 4};
+  return {16, 4};
+}
+inline Stretches backward_stretches(int64_t m, int64_t n, int64_t rows_per_gate, bool gate, int elem_kind) {
+  const int waves = backward_shape(n, elem_kind).waves;
+  return plan_stretches(m, rows_per_gate, gate, (int64_t)device_cus() * (waves == 1 ? 8 : waves == 4 ? 2 : 1));
+}
+
+template <int KIND, int WAVES, int ITEMS>
+LaunchStatus backward_launch(const NormGateGradArgs &p, const Stretches &s, uint32_t block_dim, hipStream_t stream) {
+  const int64_t most = (int64_t)1 << 20;
+  const int64_t blocks = block_dim ? block_dim : s.count < most ? s.count : most;
+  if (s.one_gate)
+    AFIR_LAUNCH("norm_gate_backward", (norm_gate_backward<KIND, WAVES, ITEMS, true>), dim3((unsigned)blocks),
+                dim3(WAVES * 64), 0, stream, p, s);
+  else
+    AFIR_LAUNCH("norm_gate_backward", (norm_gate_backward<KIND, WAVES, ITEMS, false>), dim3((unsigned)blocks),
+                dim3(WAVES * 64), 0, stream, p, s);
+  const LaunchStatus st = after_launch();
+  if (st.code) return st;
+  const int64_t column_tiles = (p.n + 63) / 64;
+  const int64_t gates = s.one_gate && p.f && p.gate ? (p.m + p.rows_per_gate - 1) / p.rows_per_gate : 0;
+  AFIR_LAUNCH("norm_gate_join", (norm_gate_join<KIND>), dim3((unsigned)column_tiles, (unsigned)(2 + gates)),
+              dim3(kJoinWaves * 64), 0, stream, p, s, column_tiles);
+  return after_launch();
+}
+
+template <int KIND>
+LaunchStatus backward(const NormGateGradArgs &p, uint32_t block_dim, hipStream_t stream) {
+  const Stretches s = backward_stretches(p.m, p.n, p.rows_per_gate, p.f && p.gate, KIND);
+  const RowShape shape = backward_shape(p.n, KIND);
+  if (shape.waves == 1)
+    return shape.items == 1 ? backward_launch<KIND, 1, 1>(p, s, block_dim, stream)
+                            : backward_launch<KIND, 1, 2>(p, s, block_dim, stream);
+  if (shape.waves == 4)
+    return shape.items == 1   ? backward_launch<KIND, 4, 1>(p, s, block_dim, stream)
+           : shape.items == 2 ? backward_launch<KIND, 4, 2>(p, s, block_dim, stream)
+                              : backward_launch<KIND, 4, 4>(p, s, block_dim, stream);
+  if constexpr (kNormMaxColumns / Elem<KIND>::kPer16 > 2048)
+    if (shape.waves == 16) return backward_launch<KIND, 16, 4>(p, s, block_dim, stream);
+  return backward_launch<KIND, 8, 4>(p, s, block_dim, stream);
+}
+
+}  // namespace
+
+LaunchStatus launch_norm_gate_residual(const NormGateArgs &args, int elem_kind, uint32_t block_dim, hipStream_t stream) {
+  NormGateArgs p = args;
+  if (p.m < 0 || p.n < 0) return invalid("norm_gate_residual: negative extent");
+  if (p.m == 0 || p.n == 0) return ok_status();
+  if (elem_kind < kElemF32 || elem_kind > kElemBF16) return invalid("norm_gate_residual: elem_type must be 0, 1 or 2");
+  if (p.m > 0x7fffffff || p.n > kNormMaxColumns)
+    return invalid("norm_gate_residual: more than 2^31 rows or rows of more than 16384 numbers");
+  if (!p.x) return invalid("norm_gate_residual: null tensor pointer");
+  if (!p.f && !p.h) return invalid("norm_gate_residual: neither a block output nor a norm of the sum is asked for");
+  if (p.f && (!p.post_weight || !p.y)) return invalid("norm_gate_residual: f needs post_weight and y");
+  if (!p.f && (p.y || p.gate)) return invalid("norm_gate_residual: without f there is no y and no gate");
+  if (p.h && !p.pre_weight) return invalid("norm_gate_residual: h needs pre_weight");
+  if (p.rows_per_gate < 1) return invalid("norm_gate_residual: rows_per_gate must be positive");
+  if (!(p.eps >= 0.f)) return invalid("norm_gate_residual: eps must not be negative");
+  const int64_t most = ((int64_t)1 << 46) / p.m;
+  for (int64_t ld : {p.ld_x, p.f ? p.ld_f : p.n, p.gate ? p.ld_gate : p.n, p.y ? p.ld_y : p.n, p.h ? p.ld_h : p.n})
+    if (ld < p.n || ld > most) return invalid("norm_gate_residual: row stride below the row's length or out of range");
+  const uintptr_t elem = elem_kind == kElemF32 ? 4 : 2;
+  for (const void *q : {p.x, p.f, p.gate, p.post_weight, p.pre_weight, (const void *)p.y, (const void *)p.h})
+    if (reinterpret_cast<uintptr_t>(q) % elem) return invalid("norm_gate_residual: tensor off its element's alignment");
+  p.inv_n = (float)(1.0 / (double)p.n);
+  switch (elem_kind) {
+    case kElemF32: return forward<kElemF32>(p, block_dim, stream);
+    case kElemF16: return forward<kElemF16>(p, block_dim, stream);
+    default: return forward<kElemBF16>(p, block_dim, stream);
+  }
+}
+
+size_t norm_gate_backward_workspace(int64_t m, int64_t n, int64_t rows_per_gate, bool gate, int elem_kind) {
+  if (m <= 0 || n <= 0 || rows_per_gate < 1) return 0;
+  return (size_t)backward_stretches(m, n, rows_per_gate, gate, elem_kind).count * (size_t)n * 2 * sizeof(float);
+}
+
+LaunchStatus launch_norm_gate_residual_backward(const NormGateGradArgs &args, int elem_kind, uint32_t block_dim,
+                                                hipStream_t stream) {
+  NormGateGradArgs p = args;
+  if (p.m < 0 || p.n < 0) return invalid("norm_gate_residual_backward: negative extent");
+  if (elem_kind < kElemF32 || elem_kind > kElemBF16)
+    return invalid("norm_gate_residual_backward: elem_type must be 0, 1 or 2");
+  if (p.m == 0 || p.n == 0) return invalid("norm_gate_residual_backward: empty tensors have no gradients to write");
+  if (p.m > 0x7fffffff || p.n > kNormMaxColumns)
+    return invalid("norm_gate_residual_backward: more than 2^31 rows or rows of more than 16384 numbers");
+  if (!p.f && !p.dh) return invalid("norm_gate_residual_backward: neither a block output nor a norm of the sum is given");
+  if (!p.dx || (!p.dy && !p.dh)) return invalid("norm_gate_residual_backward: null tensor pointer");
+  if (p.dh && (!p.y || !p.pre_weight || !p.dpre_weight))
+    return invalid("norm_gate_residual_backward: dh needs y, pre_weight and dpre_weight");
+  if (p.f && (!p.post_weight || !p.df || !p.dpost_weight))
+    return invalid("norm_gate_residual_backward: f needs post_weight, df and dpost_weight");
+  if (!p.f && p.gate) return invalid("norm_gate_residual_backward: without f there is no gate");
+  if (!p.gate != !p.dgate) return invalid("norm_gate_residual_backward: gate and dgate go together");
+  if (!p.partial) return invalid("norm_gate_residual_backward: null workspace");
+  if (p.rows_per_gate < 1) return invalid("norm_gate_residual_backward: rows_per_gate must be positive");
+  if (!(p.eps >= 0.f)) return invalid("norm_gate_residual_backward: eps must not be negative");
+  const int64_t most = ((int64_t)1 << 46) / p.m;
+  for (int64_t ld : {p.dy ? p.ld_dy : p.n, p.dh ? p.ld_dh : p.n, p.dh ? p.ld_y : p.n, p.f ? p.ld_f : p.n,
+                     p.gate ? p.ld_gate : p.n, p.ld_dx, p.f ? p.ld_df : p.n})
+    if (ld < p.n || ld > most)
+      return invalid("norm_gate_residual_backward: row stride below the row's length or out of range");
+  const uintptr_t elem = elem_kind == kElemF32 ? 4 : 2;
+  for (const void *q : {p.dy, p.dh, p.y, p.f, p.gate, p.post_weight, p.pre_weight, (const void *)p.dx, (const void *)p.df,
+                        (const void *)p.dpost_weight, (const void *)p.dgate, (const void *)p.dpre_weight})
+    if (reinterpret_cast<uintptr_t>(q) % elem)
+      return invalid("norm_gate_residual_backward: tensor off its element's alignment");
+  if (reinterpret_cast<uintptr_t>(p.partial) % 4) return invalid("norm_gate_residual_backward: workspace off a 4-byte boundary");
+  p.inv_n = (float)(1.0 / (double)p.n);
+  switch (elem_kind) {
+    case kElemF32: return backward<kElemF32>(p, block_dim, stream);
+    case kElemF16: return backward<kElemF16>(p, block_dim, stream);
+    default: return backward<kElemBF16>(p, block_dim, stream);
+  }
+}
+
+}  // namespace afir

@@ -36,6 +36,12 @@ EXPORTED_SYMBOLS = [
     "afir_hip_launch_relu_broadcast_add_transpose",
     "afir_hip_launch_gather_scale_shift",
     "afir_hip_launch_matmul_add_leakyrelu",
+    "afir_hip_launch_mxfp4_quantize",
+    "afir_hip_launch_mxfp4_matmul_add_leakyrelu",
+    "afir_hip_mxfp4_matmul_workspace_bytes",
+    "afir_hip_launch_norm_gate_residual",
+    "afir_hip_launch_norm_gate_residual_backward",
+    "afir_hip_norm_gate_residual_backward_workspace_bytes",
     "afir_hip_kernel_count",
     "afir_hip_kernel_info",
     "afir_hip_find_kernel",
@@ -79,10 +85,17 @@ def load():
                        ("afir_hip_launch_broadcast_add_reducesum_noalloc", 5),
                        ("afir_hip_launch_relu_broadcast_add_transpose", 5),
                        ("afir_hip_launch_gather_scale_shift", 7),
-                       ("afir_hip_launch_matmul_add_leakyrelu", 6)]:
+                       ("afir_hip_launch_matmul_add_leakyrelu", 6),
+                       ("afir_hip_launch_mxfp4_quantize", 6),
+                       ("afir_hip_launch_mxfp4_matmul_add_leakyrelu", 8),
+                       ("afir_hip_launch_norm_gate_residual", 9),
+                       ("afir_hip_launch_norm_gate_residual_backward", 14)]:
         fn = getattr(L, name)
         fn.restype = u32
         fn.argtypes = [u32, vp] + [vp] * nptr
+    for name in ("afir_hip_mxfp4_matmul_workspace_bytes", "afir_hip_norm_gate_residual_backward_workspace_bytes"):
+        getattr(L, name).restype = ctypes.c_size_t
+        getattr(L, name).argtypes = [vp]
     L.afir_hip_kernel_count.restype = ctypes.c_int
     L.afir_hip_kernel_info.restype = ctypes.POINTER(_KernelInfo)
     L.afir_hip_kernel_info.argtypes = [ctypes.c_int]
@@ -242,6 +255,279 @@ def matmul_add_leakyrelu(a, b, bias, alpha=0.01, out=None, block_dim=0, stream=N
                       [a.data_ptr(), b.data_ptr(), bias.data_ptr(), out.data_ptr(), 0],
                       pack_tiling(m, k, n, f32_bits(alpha))))
     return out
+
+
+# ---- four-bit block products, and the norms around a residual block ------------
+#
+# Unlike the families above these take tensors of any of the three float types and rows
+# with a stride, launch on the device of their tensors, and check every tensor against the
+# others before they launch.
+
+_ELEM_TYPES = None
+
+
+def _elem_type(dtype, what):
+    global _ELEM_TYPES
+    if _ELEM_TYPES is None:
+        import torch
+        _ELEM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    code = _ELEM_TYPES.get(dtype)
+    if code is None:
+        raise AfirHipError(f"{what}: expected float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _on(t, device, what):
+    """A tensor on the device that the call's first tensor is on."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise AfirHipError(f"{what}: expected a device tensor")
+    if device is not None and t.device != device:
+        raise AfirHipError(f"{what}: on {t.device}, the call's first tensor is on {device}")
+    return t
+
+
+def _rows(t, shape, dtype, device, what):
+    """A matrix of rows that may have a stride; returns the stride in elements."""
+    _on(t, device, what)
+    if t.dtype != dtype:
+        raise AfirHipError(f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise AfirHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    ld, unit = t.stride()
+    if unit != 1 and shape[1] > 1:
+        raise AfirHipError(f"{what}: the numbers of a row must be adjacent")
+    if ld < shape[1]:
+        if shape[0] > 1:
+            raise AfirHipError(f"{what}: rows must not overlap")
+        return shape[1]   # one row: its stride means nothing
+    return ld
+
+
+def _dense(t, shape, dtype, device, what):
+    _on(t, device, what)
+    if t.dtype != dtype:
+        raise AfirHipError(f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise AfirHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise AfirHipError(f"{what}: expected a contiguous tensor")
+    return t
+
+
+def _launch_on(device, symbol, block_dim, stream, tensors, workspace, tiling):
+    """Launch with `device` current; tensors may be None.  The stream is the caller's or
+    the current one of that device."""
+    import torch
+    L = load()
+    ptrs = [None if t is None else t.data_ptr() for t in tensors]
+    ws = None if workspace is None else workspace.data_ptr()
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            st = stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
+            rc = getattr(L, symbol)(block_dim, st, *ptrs, ws, tiling)
+    else:
+        st = stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
+        rc = getattr(L, symbol)(block_dim, st, *ptrs, ws, tiling)
+    if rc:
+        _check(rc)
+
+
+def _workspace(query, tiling, device, stream):
+    """Scratch of the size that the library asks for, from torch's allocator, which hands it
+    out again only to work that follows on the stream of this call."""
+    import torch
+    size = getattr(load(), query)(tiling)
+    if not size:
+        return None
+    ws = torch.empty((size,), dtype=torch.uint8, device=device)
+    if stream is not None:
+        ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
+    return ws
+
+
+def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_values=False,
+                   block_dim=0, stream=None):
+    """x -> MXFP4 along `axis`: blocks of 32 numbers share a power of two, numbers are e2m1.
+
+    axis -1 (or 1): x is [R, K].  axis 0: x is [K, R], a weight kept input-major, say; codes
+    and scales are laid out as for its transpose.  Rows of x may have a stride.  Returns
+    (codes uint8 [R, ceil(K/32)*16], scales float8_e8m0fnu [R, ceil(K/32)]), and with
+    return_values (or values=) also the numbers they stand for, in x's shape and type.
+    Blocks that hold an infinity or a NaN read as NaN throughout."""
+    import torch
+    _on(x, None, "x")
+    if x.dim() != 2:
+        raise AfirHipError("mxfp4_quantize: x must have two dimensions")
+    if axis not in (-1, 0, 1):
+        raise AfirHipError("mxfp4_quantize: axis must be 0 or 1 (or -1)")
+    kind = _elem_type(x.dtype, "x")
+    ld = _rows(x, x.shape, x.dtype, None, "x")
+    k, r = x.shape if axis == 0 else (x.shape[1], x.shape[0])
+    kb = (k + 31) // 32
+    dev = x.device
+    if codes is None:
+        codes = torch.empty((r, kb * 16), dtype=torch.uint8, device=dev)
+    else:
+        _dense(codes, (r, kb * 16), torch.uint8, dev, "codes")
+    if scales is None:
+        scales = torch.empty((r, kb), dtype=torch.float8_e8m0fnu, device=dev)
+    else:
+        _dense(scales, (r, kb), torch.float8_e8m0fnu, dev, "scales")
+    if values is not None:
+        _dense(values, x.shape, x.dtype, dev, "values")
+    elif return_values:
+        values = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _launch_on(dev, "afir_hip_launch_mxfp4_quantize", block_dim, stream, (x, codes, scales, values), None,
+               struct.pack("<5q", x.shape[0], x.shape[1], ld, 0 if axis == 0 else 1, kind))
+    return (codes, scales) if values is None else (codes, scales, values)
+
+
+def mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias=None, alpha=0.01, out=None, out_dtype=None, k=None,
+                               block_dim=0, stream=None):
+    """out [M, N] = leakyrelu(A @ B^T + bias, alpha) with A [M, K] and B [N, K] in MXFP4, as
+    mxfp4_quantize gives them; alpha=1 leaves the sum as it is.  out_dtype (bfloat16 unless
+    out is given) is the type of bias and out.  k: K itself, where it is not a multiple of
+    32 (only checked against the codes)."""
+    import torch
+    _on(a, None, "a")
+    dev = a.device
+    if a.dim() != 2 or b.dim() != 2:
+        raise AfirHipError("mxfp4_matmul_add_leakyrelu: codes must have two dimensions")
+    m, n, kb = a.shape[0], b.shape[0], a.shape[1] // 16
+    if a.shape[1] % 16:
+        raise AfirHipError("mxfp4_matmul_add_leakyrelu: code rows must be whole blocks of 16 bytes")
+    if k is None:
+        k = kb * 32
+    elif (k + 31) // 32 != kb:
+        raise AfirHipError(f"mxfp4_matmul_add_leakyrelu: k = {k} does not have {kb} blocks")
+    _dense(a, (m, kb * 16), torch.uint8, dev, "a")
+    _dense(b, (n, kb * 16), torch.uint8, dev, "b")
+    _dense(a_scales, (m, kb), torch.float8_e8m0fnu, dev, "a_scales")
+    _dense(b_scales, (n, kb), torch.float8_e8m0fnu, dev, "b_scales")
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=dev)
+    else:
+        _dense(out, (m, n), out.dtype if out_dtype is None else out_dtype, dev, "out")
+    kind = _elem_type(out.dtype, "out")
+    if bias is not None:
+        _dense(bias, (n,), out.dtype, dev, "bias")
+    tiling = struct.pack("<5q", m, k, n, f32_bits(alpha), kind)
+    ws = _workspace("afir_hip_mxfp4_matmul_workspace_bytes", tiling, dev, stream)
+    _launch_on(dev, "afir_hip_launch_mxfp4_matmul_add_leakyrelu", block_dim, stream,
+               (a, a_scales, b, b_scales, bias, out), ws, tiling)
+    return out
+
+
+def _gate_rows(gate, m, n, rows_per_gate, dtype, dev):
+    """(rows_per_gate, row stride) of a gate [G, N] or [N] for m rows."""
+    if gate is None:
+        return max(m, 1), n
+    _on(gate, dev, "gate")
+    if gate.dim() == 1:
+        gate = gate.unsqueeze(0)
+    if gate.dim() != 2:
+        raise AfirHipError("gate: expected one or two dimensions")
+    g = gate.shape[0]
+    if rows_per_gate is None:
+        rows_per_gate = max(m, 1) if g == 1 else 1
+    if rows_per_gate < 1 or -(-m // rows_per_gate) != g:
+        raise AfirHipError(f"gate: {g} rows of {rows_per_gate} do not cover {m} rows")
+    return rows_per_gate, _rows(gate, (g, n), dtype, dev, "gate")
+
+
+def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, residual_scale=1.0, eps=1e-6,
+                       rows_per_gate=None, y=None, h=None, block_dim=0, stream=None):
+    """The end of one residual block and the start of the next, in one pass:
+
+        y = residual_scale * x + gate * rmsnorm(f) * post_weight        h = rmsnorm(y) * pre_weight
+
+    x, f [M, N] (rows may have a stride), weights [N], gate [G, N] or [N]: row i takes gate
+    row i // rows_per_gate (None: one gate row for all rows, or one each).  Without f, y is x
+    (the norm ahead of the first block); without pre_weight there is no h.  Returns (y, h).
+    y=x and h=f work in place."""
+    import torch
+    _on(x, None, "x")
+    if x.dim() != 2:
+        raise AfirHipError("norm_gate_residual: x must have two dimensions")
+    dev, dtype = x.device, x.dtype
+    kind = _elem_type(dtype, "x")
+    m, n = shape = x.shape
+    ld_x = _rows(x, shape, dtype, None, "x")
+    ld_f = ld_gate = ld_y = ld_h = n
+    if f is None:
+        if post_weight is not None or gate is not None or y is not None or pre_weight is None:
+            raise AfirHipError("norm_gate_residual: without f only x and pre_weight are used")
+        rows_per_gate = max(m, 1)
+    else:
+        ld_f = _rows(f, shape, dtype, dev, "f")
+        _dense(post_weight, (n,), dtype, dev, "post_weight")
+        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, dev)
+        if y is None:
+            y = torch.empty(shape, dtype=dtype, device=dev)
+        ld_y = _rows(y, shape, dtype, dev, "y")
+    if pre_weight is not None:
+        _dense(pre_weight, (n,), dtype, dev, "pre_weight")
+        if h is None:
+            h = torch.empty(shape, dtype=dtype, device=dev)
+        ld_h = _rows(h, shape, dtype, dev, "h")
+    elif h is not None:
+        raise AfirHipError("norm_gate_residual: h needs pre_weight")
+    _launch_on(dev, "afir_hip_launch_norm_gate_residual", block_dim, stream,
+               (x, f, post_weight, gate, pre_weight, y, h), None,
+               struct.pack("<11q", m, n, rows_per_gate, ld_x, ld_f, ld_gate, ld_y, ld_h, f32_bits(residual_scale),
+                           f32_bits(eps), kind))
+    return (x if f is None else y), h
+
+
+def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, pre_weight=None, residual_scale=1.0,
+                                eps=1e-6, rows_per_gate=None, block_dim=0, stream=None):
+    """The gradients (dx, df, dpost_weight, dgate, dpre_weight) of norm_gate_residual from
+    those of its results and the y it returned; None where it had no such input.  dy None:
+    zero.  dh, pre_weight None: the call had no h (y is not read then)."""
+    import torch
+    _on(y, None, "y")
+    if y.dim() != 2:
+        raise AfirHipError("norm_gate_residual_backward: y must have two dimensions")
+    dev, dtype = y.device, y.dtype
+    kind = _elem_type(dtype, "y")
+    m, n = shape = y.shape
+    if m == 0 or n == 0:
+        raise AfirHipError("norm_gate_residual_backward: empty tensors have no gradients to write")
+    ld_y = _rows(y, shape, dtype, None, "y")
+    ld_dy = ld_dh = ld_f = ld_gate = n
+    if (dh is None) != (pre_weight is None):
+        raise AfirHipError("norm_gate_residual_backward: dh and pre_weight go together")
+    if dh is None and dy is None:
+        raise AfirHipError("norm_gate_residual_backward: dy or dh is needed")
+    if dh is None and f is None:
+        raise AfirHipError("norm_gate_residual_backward: f or dh is needed")
+    if dy is not None:
+        ld_dy = _rows(dy, shape, dtype, dev, "dy")
+    df = dpost = dgate = dpre = None
+    if dh is not None:
+        ld_dh = _rows(dh, shape, dtype, dev, "dh")
+        _dense(pre_weight, (n,), dtype, dev, "pre_weight")
+        dpre = torch.empty((n,), dtype=dtype, device=dev)
+    if f is None:
+        if post_weight is not None or gate is not None:
+            raise AfirHipError("norm_gate_residual_backward: post_weight and gate need f")
+        rows_per_gate = m
+    else:
+        ld_f = _rows(f, shape, dtype, dev, "f")
+        _dense(post_weight, (n,), dtype, dev, "post_weight")
+        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, dev)
+        df = torch.empty(shape, dtype=dtype, device=dev)
+        dpost = torch.empty((n,), dtype=dtype, device=dev)
+        if gate is not None:
+            dgate = torch.empty(gate.shape, dtype=dtype, device=dev)
+    dx = torch.empty(shape, dtype=dtype, device=dev)
+    tiling = struct.pack("<13q", m, n, rows_per_gate, ld_dy, ld_dh, ld_y, ld_f, ld_gate, n, n,
+                         f32_bits(residual_scale), f32_bits(eps), kind)
+    ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, dev, stream)
+    _launch_on(dev, "afir_hip_launch_norm_gate_residual_backward", block_dim, stream,
+               (dy, dh, None if dh is None else y, f, post_weight, gate, pre_weight, dx, df, dpost, dgate, dpre), ws, tiling)
+    return dx, df, dpost, dgate, dpre
 
 
 def prepare(symbol: str, ptrs, tiling: bytes, block_dim: int = 0, stream=None):

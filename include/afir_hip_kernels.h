@@ -151,6 +151,80 @@ uint32_t afir_hip_launch_matmul_add_leakyrelu(uint32_t block_dim, void *stream,
                                               void *a, void *b, void *bias, void *out,
                                               void *workspace, void *tiling);
 
+/* ---- four-bit block products and the norms around a residual block ----------
+ * The operators of a transformer's residual block at 4-bit weights and
+ * activations.  No counterpart in the reference, and no artifact carries them
+ * by name, so they are outside the registry below; they are launched by symbol,
+ * in the same shape as the families above.  elem_type in their tiling data: 0
+ * f32, 1 f16, 2 bf16.  Rows may have a stride (ld_*, in elements, at least the
+ * row's length) where a field says so; everything else is densely packed.
+ * Tensors need the alignment of one element, codes a 16-byte boundary.
+ * Every result is the same on every call: sums are taken in a fixed order.
+ *
+ * MXFP4: 32 consecutive numbers share a scale 2^e, stored as the byte e + 127;
+ * a number is code * 2^e, the code e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6, sign in bit
+ * 3), two to a byte with the lower index in the lower four bits.
+ *
+ * Quantisation: e = floor(log2(largest magnitude of the block)) - 2, not below
+ * -127; numbers are divided by 2^e, rounded to the nearest code (ties to the
+ * even one) and limited to 6.  A block that holds an infinity or a NaN gets the
+ * scale byte 255 and zero codes: each of its numbers reads as NaN.  axis 1: x
+ * is [R,K], blocks run along its rows; axis 0: x is [K,R], blocks run down its
+ * columns.  Either way codes are [R, ceil(K/32)*16] bytes and scales
+ * [R, ceil(K/32)], with zeros for what is past K.  values (NULL: not wanted)
+ * receives the numbers the codes stand for, in x's layout and type.
+ * TilingData { int64 dim_arg0_0, dim_arg0_1 (extents of x as stored); int64 ld_x;
+ *              int64 axis; int64 elem_type }                                  */
+uint32_t afir_hip_launch_mxfp4_quantize(uint32_t block_dim, void *stream, void *x, void *codes,
+                                        void *scales, void *values, void *workspace,
+                                        void *tiling);
+
+/* out = max(v, v*alpha), v = A @ B^T + bias: A [M,K] and B [N,K] in MXFP4 along
+ * K as quantised above, bias [N] (NULL: none) and out [M,N] of elem_type.  The
+ * products of codes are exact and are added in float32 on the matrix cores
+ * (v_mfma_scale_f32_16x16x128_f8f6f4).  The scale byte 255 makes every number
+ * that its block enters a NaN.  workspace: NULL, or a device buffer on a
+ * 16-byte boundary of afir_hip_mxfp4_matmul_workspace_bytes(tiling) bytes,
+ * which lets large products run on a faster kernel; a launch leaves nothing in
+ * it that a later one reads, but launches that may overlap need one each.
+ * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (K); int64 dim_arg2_0 (N);
+ *              int64 alpha_f32_bits; int64 elem_type }                         */
+uint32_t afir_hip_launch_mxfp4_matmul_add_leakyrelu(uint32_t block_dim, void *stream, void *a,
+                                                    void *a_scales, void *b, void *b_scales,
+                                                    void *bias, void *out, void *workspace,
+                                                    void *tiling);
+size_t afir_hip_mxfp4_matmul_workspace_bytes(const void *tiling);
+
+/* y = residual_scale * x + gate * (f * rstd(f)) * post_weight
+ * h = y * rstd(y) * pre_weight           rstd(v) = 1 / sqrt(mean(v^2) + eps)
+ * per row; h is computed from the unrounded y.  x, f, y, h [M,N], weights [N],
+ * gate [ceil(M/rows_per_gate), N]: row i takes gate row i / rows_per_gate.
+ * f NULL (then also post_weight, gate and y): y is x itself, the norm ahead of
+ * the first block.  pre_weight NULL (then also h): no second norm.  gate NULL:
+ * 1.  y may be x and h may be f.  N at most 16384.
+ * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;
+ *              int64 ld_x, ld_f, ld_gate, ld_y, ld_h;
+ *              int64 residual_scale_f32_bits; int64 eps_f32_bits; int64 elem_type } */
+uint32_t afir_hip_launch_norm_gate_residual(uint32_t block_dim, void *stream, void *x, void *f,
+                                            void *post_weight, void *gate, void *pre_weight,
+                                            void *y, void *h, void *workspace, void *tiling);
+
+/* The gradients of everything the call above read, from dy and dh and the y it
+ * wrote: dx, df [M,N], dpost_weight, dpre_weight [N], dgate like gate (densely
+ * packed).  dy NULL: zero.  dh NULL (then also y, pre_weight, dpre_weight): the
+ * call had no h.  f NULL (then also post_weight, gate and their gradients and
+ * df): it had no f.  dx may be dy and df may be f.  workspace: a device buffer
+ * of afir_hip_norm_gate_residual_backward_workspace_bytes(tiling) bytes, one
+ * for each of the launches that may overlap.
+ * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;
+ *              int64 ld_dy, ld_dh, ld_y, ld_f, ld_gate, ld_dx, ld_df;
+ *              int64 residual_scale_f32_bits; int64 eps_f32_bits; int64 elem_type } */
+uint32_t afir_hip_launch_norm_gate_residual_backward(
+    uint32_t block_dim, void *stream, void *dy, void *dh, void *y, void *f, void *post_weight,
+    void *gate, void *pre_weight, void *dx, void *df, void *dpost_weight, void *dgate,
+    void *dpre_weight, void *workspace, void *tiling);
+size_t afir_hip_norm_gate_residual_backward_workspace_bytes(const void *tiling);
+
 /* ---- registry + name-based dispatch -----------------------------------------
  * What a runner needs to bind a kernel by the name an artifact manifest
  * carries (kernel_name=..., lib/Runtime/Artifact/VecCubeArtifactBackend.cpp:62-106)

@@ -1,0 +1,227 @@
+"""MXFP4 quantisation and products on the GPU against the float64 oracle."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import block_oracle as O
+from tests import block_cases as B
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def H(pkg):
+    from ascend_mlir_amd import hip_kernels
+    hip_kernels.load()
+    assert torch.cuda.is_available(), "no GPU visible"
+    return hip_kernels
+
+
+def check_quantize(H, x, axis, **kw):
+    """Codes, scales and values are exact: no tolerance."""
+    want = O.quantize(B.numbers(x) if axis else B.numbers(x).T)
+    codes, scales, values = H.mxfp4_quantize(x, axis=axis, return_values=True, **kw)
+    torch.cuda.synchronize()
+    assert np.array_equal(scales.view(torch.uint8).cpu().numpy(), want[1])
+    assert np.array_equal(codes.cpu().numpy(), want[0])
+    got = B.numbers(values)
+    back = want[2] if axis else want[2].T
+    assert np.array_equal(got, back, equal_nan=True)
+    fine = ~np.isnan(back)
+    assert np.array_equal(np.signbit(got[fine]), np.signbit(back[fine]))
+    two = H.mxfp4_quantize(x, axis=axis, **kw)          # without the values: the same codes
+    assert len(two) == 2 and torch.equal(two[0], codes) and torch.equal(two[1].view(torch.uint8), scales.view(torch.uint8))
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("axis", [1, 0])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 32), (3, 31), (5, 33), (64, 64), (7, 1000), (130, 257), (1, 8192),
+                                   (300, 129), (33, 2050), (2, 5)])
+def test_quantize(H, kind, axis, shape):
+    rng = np.random.default_rng(shape[0] * 1000 + shape[1])
+    x = rng.normal(size=shape) * np.exp2(rng.integers(-12, 8, (shape[0], 1)))
+    x[rng.random(shape) < 0.1] = 0
+    x[rng.random(shape[0]) < 0.2] = 0
+    check_quantize(H, B.tensor(x, kind, "cuda"), axis)
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("axis", [1, 0])
+def test_quantize_ties_and_special_numbers(H, kind, axis):
+    t = B.TYPES[kind]
+    info = torch.finfo(t)
+    grid = np.concatenate([np.arange(0, 33) / 4, [0.126, 0.2499, 1.2499, 5.0001, 7.99]])
+    rows = []
+    for e in (0, 3, -5, -9):
+        block = np.resize(grid, 64) * np.exp2(float(e)) * np.resize([1, -1, 1], 64)
+        block[31] = block[63] = 4 * np.exp2(float(e))
+        rows.append(block)
+    x = B.tensor(np.array(rows), kind, "cpu")
+    extra = torch.zeros((9, 64), dtype=t)
+    extra[0, :] = -0.0
+    extra[1, 5], extra[1, 40] = float("inf"), 1.0
+    extra[2, 5], extra[2, 40] = float("nan"), -3.0
+    extra[3, 63], extra[3, 62] = -float("inf"), info.max
+    extra[4, :] = info.max
+    extra[5, :] = info.smallest_normal
+    extra[6, :] = info.smallest_normal * info.eps      # the smallest subnormal
+    extra[6, 3] *= 3
+    extra[7, 1], extra[7, 33] = info.smallest_normal * 1.5, info.smallest_normal * 4
+    extra[8, ::2], extra[8, 1::2] = -info.max, info.smallest_normal
+    x = torch.cat([x, extra]).cuda()
+    check_quantize(H, x if axis else x.t().contiguous(), axis)
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+def test_quantize_every_16_bit_number(H, kind):
+    if kind == "f32":
+        bits = torch.arange(0, 1 << 16, dtype=torch.int32) * 65537 + 12345    # spread over the float32 patterns
+        x = bits.view(torch.float32)
+    else:
+        x = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(B.TYPES[kind])
+    # neighbours in value share a block, and every number meets a block of far larger ones too
+    x = torch.cat([x.reshape(-1, 64), x.reshape(64, -1).t()]).cuda()
+    check_quantize(H, x.contiguous(), 1)
+    check_quantize(H, x.t().contiguous(), 0)
+
+
+@pytest.mark.parametrize("axis", [1, 0])
+def test_quantize_rows_with_a_stride_and_off_alignment(H, axis):
+    rng = np.random.default_rng(5)
+    for kind in B.TYPES:
+        wide = B.tensor(rng.normal(size=(65, 403)), kind, "cuda")
+        check_quantize(H, wide[:, 1:258], axis)          # rows start off every boundary but an element's
+        check_quantize(H, wide[3:4, 2:100], axis)
+        check_quantize(H, wide[::2, :64], axis)
+
+
+def test_quantize_into_given_tensors_and_few_workgroups(H):
+    x = torch.randn(40, 200, device="cuda", dtype=torch.bfloat16)
+    guard = torch.full((42, 7 * 16), 77, dtype=torch.uint8, device="cuda")
+    scales = torch.full((42, 7), 77, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    values = torch.full((42, 200), 77.0, dtype=torch.bfloat16, device="cuda")
+    want = H.mxfp4_quantize(x, return_values=True)
+    got = H.mxfp4_quantize(x, codes=guard[1:41], scales=scales[1:41], values=values[1:41], block_dim=1)
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for t in (guard, scales.view(torch.uint8), values):   # the rows around are left as they were
+        assert (t[0] == 77).all() and (t[41] == 77).all()
+    xt = x.t().contiguous()
+    got = H.mxfp4_quantize(xt, axis=0, codes=guard[1:41], scales=scales[1:41], block_dim=2)
+    assert torch.equal(got[0], want[0])
+    assert (guard[0] == 77).all() and (guard[41] == 77).all()
+
+
+def test_quantize_refuses(H):
+    x = torch.zeros(8, 64, device="cuda")
+    for bad, word in ((dict(x=x.int()), "float32"), (dict(x=x[0]), "two dimensions"), (dict(x=x, axis=2), "axis"),
+                      (dict(x=x.t()), "adjacent"), (dict(x=x[:1].expand(8, 64)), "overlap"),
+                      (dict(x=x, codes=torch.zeros(8, 31, dtype=torch.uint8, device="cuda")), "shape"),
+                      (dict(x=x, codes=torch.zeros(8, 32, device="cuda")), "uint8"),
+                      (dict(x=x, scales=torch.zeros(8, 2, dtype=torch.uint8, device="cuda")), "e8m0"),
+                      (dict(x=x, values=torch.zeros(8, 64, device="cuda").half()), "float32"),
+                      (dict(x=x, values=torch.zeros(64, 8, device="cuda").t()), "contiguous")):
+        with pytest.raises(H.AfirHipError, match=word):
+            H.mxfp4_quantize(**bad)
+
+
+# ---- products ----
+
+def operand(rng, rows, k, spread=3):
+    kb = -(-k // 32)
+    codes = rng.integers(0, 256, (rows, kb * 16), dtype=np.uint8)
+    scales = (127 + rng.integers(-spread, spread + 1, (rows, kb))).astype(np.uint8)
+    return codes, scales
+
+
+def check_matmul(H, m, n, k, kind, bias=True, alpha=0.01, seed=0, **kw):
+    rng = np.random.default_rng(seed + 7 * m + 11 * n + 13 * k)
+    (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
+    size_of_sum = np.sqrt(k) * 10
+    bias_t = B.tensor(rng.normal(size=n) * size_of_sum, kind, "cuda") if bias else None
+    want, size = O.matmul(O.decode(ac, asc), O.decode(bc, bsc), None if bias_t is None else B.numbers(bias_t), alpha)
+    dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
+    guard = torch.full((m + 2, n), 77.0, dtype=B.TYPES[kind], device="cuda")
+    got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2], dev[3].view(torch.float8_e8m0fnu),
+                                       bias_t, alpha=alpha, out=guard[1:m + 1] if n % 8 == 0 else None,
+                                       out_dtype=B.TYPES[kind], **kw)
+    torch.cuda.synchronize()
+    # numbers of a block are multiples of 1/4 up to 36, their sum over a block is exact in float32; what rounds is the
+    # sum over ceil(k / 32) blocks, the joining of eight partial sums, the bias and the slope
+    B.close(got, want, size, kind, -(-k // 32) + 10)
+    if n % 8 == 0:
+        assert (guard[0] == 77).all() and (guard[m + 1] == 77).all()
+    return got
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 32), (1, 40, 33), (3, 31, 96), (15, 257, 512), (16, 32, 544),
+                                   (17, 48, 1056), (33, 100, 4096), (48, 72, 8192), (64, 33, 640), (65, 17, 256),
+                                   (130, 264, 288)])
+def test_matmul(H, kind, m, n, k):
+    check_matmul(H, m, n, k, kind)
+    check_matmul(H, m, n, k, kind, bias=False, alpha=1.0)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 24, 2048), (64, 520, 1000), (200, 1032, 776)])
+def test_matmul_on_few_workgroups(H, m, n, k):
+    a = check_matmul(H, m, n, k, "bf16", block_dim=3)
+    assert torch.equal(a, check_matmul(H, m, n, k, "bf16"))
+
+
+def test_matmul_without_depth_is_the_bias(H):
+    a = torch.zeros((5, 0), dtype=torch.uint8, device="cuda")
+    b = torch.zeros((24, 0), dtype=torch.uint8, device="cuda")
+    s = lambda t: torch.zeros((t.shape[0], 0), dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    bias = torch.randn(24, device="cuda").bfloat16()
+    got = H.mxfp4_matmul_add_leakyrelu(a, s(a), b, s(b), bias, alpha=0.5)
+    want = torch.maximum(bias.float(), bias.float() * 0.5).bfloat16().expand(5, 24)
+    assert torch.equal(got, want)
+    assert not H.mxfp4_matmul_add_leakyrelu(a, s(a), b, s(b)).any()
+
+
+def test_matmul_keeps_nan_to_the_rows_and_columns_that_hold_it(H):
+    rng = np.random.default_rng(3)
+    for m, n, k in ((5, 40, 320), (70, 80, 1056)):
+        (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
+        asc[2, -1] = 255
+        bsc[7, 0] = 255
+        bc[7, :16] = 0                       # as quantisation writes such a block
+        dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
+        got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2],
+                                           dev[3].view(torch.float8_e8m0fnu), out_dtype=torch.float32)
+        want = np.zeros((m, n), dtype=bool)
+        want[2, :] = want[:, 7] = True
+        assert np.array_equal(np.isnan(got.cpu().numpy()), want)
+
+
+def test_matmul_scales_at_their_ends(H):
+    # scale bytes 0 and 254: the sums stay in range because the other operand's scales answer them
+    k, m, n = 576, 9, 33
+    rng = np.random.default_rng(4)
+    (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
+    asc[:], bsc[:] = 0, 254
+    asc[:, ::2], bsc[:, ::2] = 250, 4
+    want, size = O.matmul(O.decode(ac, asc), O.decode(bc, bsc), None, 1.0)
+    dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
+    got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2], dev[3].view(torch.float8_e8m0fnu),
+                                       alpha=1.0, out_dtype=torch.float32)
+    B.close(got, want, size, "f32", k // 32 + 10)
+
+
+def test_matmul_refuses(H):
+    u8 = dict(dtype=torch.uint8, device="cuda")
+    a, b = torch.zeros(4, 32, **u8), torch.zeros(8, 32, **u8)
+    sa, sb = (torch.zeros(t.shape[0], 2, **u8).view(torch.float8_e8m0fnu) for t in (a, b))
+    bias = torch.zeros(8, device="cuda", dtype=torch.bfloat16)
+    H.mxfp4_matmul_add_leakyrelu(a, sa, b, sb, bias, k=63)
+    for args, kw, word in (((a, sa, b[:, :16], sb), {}, "shape"), ((a, sa, b, sa), {}, "shape"),
+                           ((a[:, :24], sa, b, sb), {}, "whole blocks"), ((a.int(), sa, b, sb), {}, "uint8"),
+                           ((a, sa.view(torch.uint8), b, sb), {}, "e8m0"), ((a, sa, b, sb, bias.float()), {}, "bfloat16"),
+                           ((a, sa, b, sb, bias[:4]), {}, "shape"), ((a, sa, b, sb), dict(k=65), "blocks"),
+                           ((a, sa, b, sb), dict(k=32), "blocks"), ((a, sa, b, sb), dict(out_dtype=torch.int32), "float32"),
+                           ((a, sa, b, sb), dict(out=bias.reshape(1, 8)), "shape"),
+                           ((torch.zeros(32, 4, **u8).t(), sa, b, sb), {}, "contiguous"),
+                           ((torch.zeros(4 * 32 + 1, **u8)[1:].view(4, 32), sa, b, sb), {}, "16-byte")):
+        with pytest.raises(H.AfirHipError, match=word):
+            H.mxfp4_matmul_add_leakyrelu(*args, **kw)
