@@ -46,6 +46,7 @@ KERNEL_SOURCES = [
     ("kernels/matmul_layouts.hip", []),
     ("kernels/mxfp4_quantize.hip", []),
     ("kernels/mxfp4_matmul.hip", []),
+    ("kernels/mxfp4_matmul_dma.hip", []),
     ("kernels/norm_gate.hip", []),
     ("kernels/region.hip", STRICT),
     ("target/region_program.cpp", []),

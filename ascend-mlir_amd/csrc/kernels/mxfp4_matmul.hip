@@ -1,42 +1,13 @@
 // out = leakyrelu(A B^T + bias) with A [M, K] and B [N, K] in MXFP4 (mxfp4.h) along K.
-//
-// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes and applies the block
-// scales: lane l holds row l % 16, the 32 codes (16 bytes) of one block, and that block's scale
-// byte; the four lanes of a row hold four different blocks.  Which four is free as long as both
-// operands agree, since a sum over blocks has no order that matters.  Products of two codes are
-// multiples of 1/4 up to 36, and the instruction adds them in float32.  B is the row operand, so a
-// lane's four accumulators are four consecutive columns of one output row.
-#include <type_traits>
-
-#include "kernels.h"
-#include "mxfp4.h"
+// Products of few rows; the dispatch of all of them.
+#include "mxfp4_mfma.h"
 
 namespace afir {
 
 namespace {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
-
-constexpr int kFp4 = 4;   // the format number of e2m1 in the instruction's two format fields
-
-// scale byte BA of `sa` and BB of `sb` go with these 16 bytes
-template <int BB, int BA>
-__device__ __forceinline__ f32x4 mfma_fp4(u32x4 b, u32x4 a, f32x4 c, uint32_t sb, uint32_t sa) {
-  const i32x8 b8 = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  const i32x8 a8 = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b8, a8, c, kFp4, kFp4, BB, (int)sb, BA, (int)sa);
-}
-
-struct MxOperands {
-  const unsigned char *a, *b;         // codes, kb * 16 bytes a row
-  const uint8_t *a_scales, *b_scales; // kb bytes a row
-  const void *bias;                   // of the output's type, or null
-  void *out;
-  int m, n, kb;
-  float alpha;
-};
+constexpr int64_t kMaxExtent = 0x7ffffe00;   // extents and what a tile rounds them up to are 32-bit
 
 template <int KIND>
 __device__ __forceinline__ void finish_one(const MxOperands &p, int m, int n, float v) {
@@ -147,7 +118,8 @@ LaunchStatus rows_launch(const MxOperands &p, uint32_t block_dim, hipStream_t st
 }
 
 template <int KIND>
-LaunchStatus matmul(const MxOperands &p, uint32_t block_dim, hipStream_t stream) {
+LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hipStream_t stream) {
+  if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
   if (p.m <= 16) return rows_launch<1, 2, KIND>(p, block_dim, stream);
   if (p.m <= 32) return rows_launch<2, 2, KIND>(p, block_dim, stream);
   return rows_launch<4, 2, KIND>(p, block_dim, stream);
@@ -155,15 +127,22 @@ LaunchStatus matmul(const MxOperands &p, uint32_t block_dim, hipStream_t stream)
 
 }  // namespace
 
-size_t mxfp4_matmul_workspace(int64_t, int64_t, int64_t) { return 0; }
+size_t mxfp4_matmul_workspace(int64_t m, int64_t k, int64_t n) {
+  if (m <= 0 || n <= 0 || k <= 0 || m > kMaxExtent || n > kMaxExtent || k > kMaxExtent) return 0;
+  const int kb = (int)((k + kMxBlock - 1) / kMxBlock);
+  MxOperands p{};
+  p.m = (int)m;
+  p.n = (int)n;
+  p.kb = kb;
+  return mxfp4_dma_supported(p) ? mxfp4_dma_workspace(m, kb, n) : 0;
+}
 
 LaunchStatus launch_mxfp4_matmul(const void *a, const void *a_scales, const void *b, const void *b_scales,
                                  const void *bias, void *out, int64_t m, int64_t k, int64_t n, float alpha,
                                  int elem_kind, void *workspace, uint32_t block_dim, hipStream_t stream) {
-  (void)workspace;
   if (m < 0 || k < 0 || n < 0) return invalid("mxfp4_matmul_add_leakyrelu: negative extent");
   if (m == 0 || n == 0) return ok_status();
-  if (m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) return invalid("mxfp4_matmul_add_leakyrelu: extent above 2^31");
+  if (m > kMaxExtent || n > kMaxExtent || k > kMaxExtent) return invalid("mxfp4_matmul_add_leakyrelu: extent above 2^31");
   if (!out || (k > 0 && (!a || !a_scales || !b || !b_scales)))
     return invalid("mxfp4_matmul_add_leakyrelu: null tensor pointer");
   if (elem_kind < kElemF32 || elem_kind > kElemBF16)
@@ -171,15 +150,16 @@ LaunchStatus launch_mxfp4_matmul(const void *a, const void *a_scales, const void
   const uintptr_t elem = elem_kind == kElemF32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) % elem)
     return invalid("mxfp4_matmul_add_leakyrelu: tensor off its element's alignment");
+  if (!aligned16(workspace)) return invalid("mxfp4_matmul_add_leakyrelu: workspace off a 16-byte boundary");
   if (!aligned16(a) || !aligned16(b))
     return invalid("mxfp4_matmul_add_leakyrelu: codes must start on a 16-byte boundary");
   const MxOperands p{static_cast<const unsigned char *>(a), static_cast<const unsigned char *>(b),
                      static_cast<const uint8_t *>(a_scales), static_cast<const uint8_t *>(b_scales), bias, out,
                      (int)m, (int)n, (int)((k + kMxBlock - 1) / kMxBlock), alpha};
   switch (elem_kind) {
-    case kElemF32: return matmul<kElemF32>(p, block_dim, stream);
-    case kElemF16: return matmul<kElemF16>(p, block_dim, stream);
-    default: return matmul<kElemBF16>(p, block_dim, stream);
+    case kElemF32: return matmul<kElemF32>(p, workspace, block_dim, stream);
+    case kElemF16: return matmul<kElemF16>(p, workspace, block_dim, stream);
+    default: return matmul<kElemBF16>(p, workspace, block_dim, stream);
   }
 }
 
