@@ -6,7 +6,7 @@ namespace afir {
 
 namespace {
 
-typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
 constexpr int64_t kMaxExtent = 0x7ffffe00;   // extents and what a tile rounds them up to are 32-bit
 
 template <int KIND>
@@ -17,18 +17,47 @@ __device__ __forceinline__ void finish_one(const MxOperands &p, int m, int n, fl
 }
 
 // Few rows of A (MT tiles of 16): the time is that of reading B.  A workgroup owns 16 * NT
-// columns and its eight wavefronts deal the blocks of K out among themselves, 16 blocks at a time:
-// lane group g of a wavefront takes blocks 4g .. 4g + 3, so a row's scales are one 32-bit load and
-// its codes four 16-byte loads.  Everything of a step is requested before the first product.  The
-// eight partial sums meet in LDS and are added in a fixed order.
+// columns and its eight wavefronts deal the blocks of K out among themselves, 16 blocks (256 bytes
+// of a row) at a step.  Of a step, lane group g of a wavefront takes blocks g, 4 + g, 8 + g and
+// 12 + g: each of the four loads then covers 64 adjacent bytes of each of the 16 rows, a quarter of
+// the segments that four adjacent blocks per lane would touch (that was the bound: 48 rows of A
+// 15.9 us, one row 9.1).  The row's sixteen scales come as one 16-byte load and are shifted to the
+// lane's byte.  Everything of a step is requested before the first product, where the registers
+// allow it (kAhead) the next step's too.  The eight partial sums meet in LDS and are added in a
+// fixed order.
 constexpr int kRowsWaves = 8;
+
+// 16 rows' codes and scales of one step
+struct RowsPiece {
+  u32x4 w[4], s;
+  // all 16 blocks of the step are there
+  __device__ __forceinline__ void load(const unsigned char *codes, const uint8_t *scales, int64_t row, int kb, int step, int g) {
+    const u32x4 *const q = reinterpret_cast<const u32x4 *>(codes + row * kb * kMxBlockBytes) + step * 16 + g;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) w[c] = q[4 * c];
+    s = *reinterpret_cast<const u32x4_any *>(scales + row * kb + step * 16);
+  }
+  // the blocks past the end: zeros, at scale 1
+  __device__ __forceinline__ void load_tail(const unsigned char *codes, const uint8_t *scales, int64_t row, int kb, int step, int g) {
+    uint32_t v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int block = step * 16 + 4 * c + g;
+      w[c] = block < kb ? reinterpret_cast<const u32x4 *>(codes + row * kb * kMxBlockBytes)[block] : u32x4{0, 0, 0, 0};
+      v[c] = (block < kb ? (uint32_t)scales[row * kb + block] : 127u) << (8 * g);
+    }
+    s = u32x4{v[0], v[1], v[2], v[3]};
+  }
+};
+
 template <int MT, int NT, int KIND>
 __global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands p, int tiles_n, int chunks_m,
                                                                      int blocks) {
   constexpr int kCols = 16 * NT, kRows = 16 * MT;
+  constexpr bool kAhead = MT + NT <= 4;
   __shared__ f32x4 part[kRowsWaves][kRows * kCols / 4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, g = lane >> 4;
-  const int64_t pitch = (int64_t)p.kb * kMxBlockBytes;
+  const int shift = 8 * g;
   for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
     // chunks of A that share columns follow one another on one XCD, whose L2 then holds the columns' B
     const int xcd = block % kNumXCD, idx = block / kNumXCD;
@@ -46,49 +75,51 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands 
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int step = wave; step * 16 < p.kb; step += kRowsWaves) {
-      const int k0 = step * 16 + 4 * g;
-      u32x4 a[MT][4], b[NT][4];
-      uint32_t sa[MT], sb[NT];
-      if (step * 16 + 16 <= p.kb) {
+    RowsPiece a[MT], b[NT], a_next[kAhead ? MT : 1], b_next[kAhead ? NT : 1];
+    auto fetch = [&](int step, RowsPiece *pa, RowsPiece *pb) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const u32x4 *q = reinterpret_cast<const u32x4 *>(p.b + row_b[j] * pitch) + k0;
+      for (int j = 0; j < NT; ++j) pb[j].load(p.b, p.b_scales, row_b[j], p.kb, step, g);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) b[j][c] = q[c];
-          sb[j] = *reinterpret_cast<const u32_any *>(p.b_scales + row_b[j] * p.kb + k0);
-        }
+      for (int i = 0; i < MT; ++i) pa[i].load(p.a, p.a_scales, row_a[i], p.kb, step, g);
+    };
+    auto multiply = [&]() {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t sb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sb[j] = b[j].s[c] >> shift;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const u32x4 *q = reinterpret_cast<const u32x4 *>(p.a + row_a[i] * pitch) + k0;
+          const uint32_t sa = a[i].s[c] >> shift;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) a[i][c] = q[c];
-          sa[i] = *reinterpret_cast<const u32_any *>(p.a_scales + row_a[i] * p.kb + k0);
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_fp4<0, 0>(b[j].w[c], a[i].w[c], acc[i][j], sb[j], sa);
         }
-      } else {   // the blocks past the end: zeros, at scale 1
-        auto fetch = [&](const unsigned char *codes, const uint8_t *scales, int64_t row, u32x4 (&w)[4], uint32_t &s) {
-          s = 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const bool in = k0 + c < p.kb;
-            w[c] = in ? reinterpret_cast<const u32x4 *>(codes + row * pitch)[k0 + c] : u32x4{0, 0, 0, 0};
-            s |= (in ? (uint32_t)scales[row * p.kb + k0 + c] : 127u) << (8 * c);
-          }
-        };
-#pragma unroll
-        for (int j = 0; j < NT; ++j) fetch(p.b, p.b_scales, row_b[j], b[j], sb[j]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) fetch(p.a, p.a_scales, row_a[i], a[i], sa[i]);
       }
+    };
+    const int whole = p.kb / 16;   // steps of 16 blocks
+    int step = wave;
+    if constexpr (kAhead) {
+      if (step < whole) fetch(step, a, b);
+      for (; step < whole; step += kRowsWaves) {
+        if (step + kRowsWaves < whole) fetch(step + kRowsWaves, a_next, b_next);
+        multiply();
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i) a[i] = a_next[i];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[i][j] = mfma_fp4<0, 0>(b[j][0], a[i][0], acc[i][j], sb[j], sa[i]);
-          acc[i][j] = mfma_fp4<1, 1>(b[j][1], a[i][1], acc[i][j], sb[j], sa[i]);
-          acc[i][j] = mfma_fp4<2, 2>(b[j][2], a[i][2], acc[i][j], sb[j], sa[i]);
-          acc[i][j] = mfma_fp4<3, 3>(b[j][3], a[i][3], acc[i][j], sb[j], sa[i]);
-        }
+        for (int j = 0; j < NT; ++j) b[j] = b_next[j];
+      }
+    } else {
+      for (; step < whole; step += kRowsWaves) {
+        fetch(step, a, b);
+        multiply();
+      }
+    }
+    if (step == whole && whole * 16 < p.kb) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) b[j].load_tail(p.b, p.b_scales, row_b[j], p.kb, step, g);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[i].load_tail(p.a, p.a_scales, row_a[i], p.kb, step, g);
+      multiply();
     }
     // part[wave]: row-major [kRows][kCols]; lane: row i * 16 + li, columns j * 16 + 4 g ..
 #pragma unroll
@@ -97,11 +128,13 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands 
       for (int j = 0; j < NT; ++j) part[wave][((i * 16 + li) * kCols + j * 16 + 4 * g) / 4] = acc[i][j];
     __syncthreads();
     for (int e = t; e < kRows * kCols; e += kRowsWaves * 64) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRowsWaves; ++w) v += reinterpret_cast<const float *>(part[w])[e];
       const int m = m0 + e / kCols, n = n0 + e % kCols;
-      if (m < p.m && n < p.n) finish_one<KIND>(p, m, n, v);
+      if (m < p.m && n < p.n) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowsWaves; ++w) v += reinterpret_cast<const float *>(part[w])[e];
+        finish_one<KIND>(p, m, n, v);
+      }
     }
     __syncthreads();
   }
@@ -122,6 +155,7 @@ LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hi
   if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
   if (p.m <= 16) return rows_launch<1, 2, KIND>(p, block_dim, stream);
   if (p.m <= 32) return rows_launch<2, 2, KIND>(p, block_dim, stream);
+  if (p.m <= 48) return rows_launch<3, 2, KIND>(p, block_dim, stream);
   return rows_launch<4, 2, KIND>(p, block_dim, stream);
 }
 

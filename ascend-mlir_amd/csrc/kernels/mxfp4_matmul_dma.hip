@@ -74,28 +74,49 @@ inline int64_t scale_units(int64_t rows) {
 inline int64_t slices_of(int64_t kb) { return (kb + kSliceBlocks - 1) / kSliceBlocks; }
 
 // scales [rows][kb] -> [slice][unit][lane][4 tiles][2]: lane l = 16 g + r holds, of row 16 i + r of the
-// unit, blocks 2g and 2g + 1 of the slice.  A's units first, then B's.
+// unit, blocks 2g and 2g + 1 of the slice.  A's units first, then B's.  A workgroup turns a unit's rows
+// of 16 slices (128 bytes each) in LDS, so that both sides move whole lines.
+constexpr int kTurnSlices = 16, kTurnPitch = kTurnSlices * kSliceBlocks + 4;
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
 __global__ __launch_bounds__(256) void mxfp4_arrange_scales(MxOperands p, int units_a, int units_b, int slices,
-                                                            u32x2 *__restrict__ out) {
-  const int64_t total = (int64_t)(units_a + units_b) * slices * 64;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    // neighbouring wavefronts take neighbouring slices of a unit: together they read whole lines
-    const int lane = (int)(i & 63);
-    const int64_t piece = i >> 6;
-    const int slice = (int)(piece % slices), unit_all = (int)(piece / slices);
+                                                            int turns, unsigned char *__restrict__ out) {
+  __shared__ __align__(16) unsigned char tile[kUnitRows * kTurnPitch];
+  const int64_t total = (int64_t)(units_a + units_b) * turns;
+  for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
+    const int unit_all = (int)(item / turns), s0 = (int)(item % turns) * kTurnSlices;
     const bool is_a = unit_all < units_a;
-    const int unit = is_a ? unit_all : unit_all - units_a, units = is_a ? units_a : units_b;
+    const int unit = is_a ? unit_all : unit_all - units_a, units = is_a ? units_a : units_b, rows = is_a ? p.m : p.n;
     const uint8_t *const s = is_a ? p.a_scales : p.b_scales;
-    const int rows = is_a ? p.m : p.n, r = lane & 15, block = slice * kSliceBlocks + 2 * (lane >> 4);
-    uint32_t w[4];
+    for (int i = threadIdx.x; i < kUnitRows * 8; i += 256) {
+      const int r = i >> 3, at = (i & 7) * 16, block = s0 * kSliceBlocks + at;
+      const int row = unit * kUnitRows + r < rows ? unit * kUnitRows + r : rows - 1;
+      const uint8_t *const q = s + (int64_t)row * p.kb + block;
+      uint32_t w[4] = {0, 0, 0, 0};   // past the end: 2^-127
+      if (block + 16 <= p.kb) {
+        const u32x4 v = *reinterpret_cast<const u32x4_any *>(q);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int row = unit * kUnitRows + t * 16 + r;
-      const uint8_t *const q = s + (int64_t)(row < rows ? row : rows - 1) * p.kb + block;
-      w[t] = (block < p.kb ? (uint32_t)q[0] : 0u) | (block + 1 < p.kb ? (uint32_t)q[1] << 8 : 0u);
+        for (int e = 0; e < 16; ++e)
+          if (block + e < p.kb) w[e / 4] |= (uint32_t)q[e] << (8 * (e & 3));
+      }
+      uint32_t *const to = reinterpret_cast<uint32_t *>(tile + r * kTurnPitch + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = w[e];
     }
-    u32x2 *const piece_out = out + (is_a ? 0 : (int64_t)units_a * slices * 64) + ((int64_t)slice * units + unit) * 64;
-    piece_out[lane] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+    __syncthreads();
+    u32x2 *const to = reinterpret_cast<u32x2 *>(out + (is_a ? 0 : (int64_t)units_a * slices * kUnitBytes));
+    for (int i = threadIdx.x; i < kTurnSlices * 64; i += 256) {
+      const int lane = i & 63, ds = i >> 6, slice = s0 + ds;
+      if (slice < slices) {
+        const unsigned char *const from = tile + (lane & 15) * kTurnPitch + ds * kSliceBlocks + 2 * (lane >> 4);
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint16_t *>(from + t * 16 * kTurnPitch);
+        to[((int64_t)slice * units + unit) * 64 + lane] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -497,10 +518,10 @@ LaunchStatus tiles_launch(const MxOperands &p, const unsigned char *scales, int 
 template <int KIND>
 LaunchStatus tiles(const MxOperands &p, void *workspace, uint32_t block_dim, hipStream_t stream) {
   const int slices = (int)slices_of(p.kb), units_a = (int)scale_units(p.m), units_b = (int)scale_units(p.n);
-  const int64_t pieces = (int64_t)(units_a + units_b) * slices;
-  const int64_t blocks = (pieces + 3) / 4, most = (int64_t)device_cus() * 16;
-  AFIR_LAUNCH("mxfp4_arrange_scales", mxfp4_arrange_scales, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0,
-              stream, p, units_a, units_b, slices, static_cast<u32x2 *>(workspace));
+  const int turns = (slices + kTurnSlices - 1) / kTurnSlices;
+  const int64_t items = (int64_t)(units_a + units_b) * turns, most = (int64_t)1 << 20;
+  AFIR_LAUNCH("mxfp4_arrange_scales", mxfp4_arrange_scales, dim3((unsigned)(items < most ? items : most)), dim3(256), 0,
+              stream, p, units_a, units_b, slices, turns, static_cast<unsigned char *>(workspace));
   const LaunchStatus st = after_launch();
   if (st.code) return st;
   const unsigned char *const scales = static_cast<const unsigned char *>(workspace);

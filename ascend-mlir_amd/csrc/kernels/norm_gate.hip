@@ -74,18 +74,24 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], float *lds, int &tur
 #pragma unroll
   for (int c = 0; c < COUNT; ++c) v[c] = wave_sum(v[c]);
   if constexpr (WAVES > 1) {
-    float *part = lds + turn * (WAVES * 4);
+    f32x4 *const part = reinterpret_cast<f32x4 *>(lds) + turn * WAVES;
     turn ^= 1;
-    if ((threadIdx.x & 63) == 0)
+    if ((threadIdx.x & 63) == 0) {
+      f32x4 mine = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < COUNT; ++c) part[wave * 4 + c] = v[c];
+      for (int c = 0; c < COUNT; ++c) mine[c] = v[c];
+      part[wave] = mine;
+    }
     __syncthreads();
+    // every 16 lanes take the WAVES sums, one each, and add them across (as wave_sum does within a row of 16)
+    const int from = threadIdx.x & 15;
+    const f32x4 one = from < WAVES ? part[from] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < COUNT; ++c) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) s += part[w * 4 + c];
-      v[c] = s;
+      v[c] = dpp_add<0xB1>(one[c]);
+      v[c] = dpp_add<0x4E>(v[c]);
+      v[c] = dpp_add<0x141>(v[c]);
+      v[c] = dpp_add<0x140>(v[c]);
     }
   }
 }
@@ -94,12 +100,13 @@ __device__ __forceinline__ float rstd_of(float sum_of_squares, float inv_n, floa
   return 1.0f / sqrtf(sum_of_squares * inv_n + eps);
 }
 
-constexpr int threads_of(int waves) { return waves == 1 ? 256 : waves * 64; }   // single-wave rows: four to a workgroup
+// forward: rows of one wavefront, which need no barrier, are four to a workgroup
+constexpr int threads_of(int waves) { return waves == 1 ? 256 : waves * 64; }
 
 template <int KIND, int WAVES, int ITEMS>
 __global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateArgs p) {
   constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64, kRowsHere = threads_of(WAVES) / kLanes;
-  __shared__ float lds[2 * WAVES * 4];
+  __shared__ __align__(16) float lds[2 * WAVES * 4];
   const int lane = threadIdx.x % kLanes, wave = lane >> 6;
   const int64_t n = p.n;
   Piece<KIND, ITEMS> post, pre;
@@ -188,10 +195,10 @@ template <int KIND>
 LaunchStatus forward(const NormGateArgs &p, uint32_t block_dim, hipStream_t stream) {
   const int64_t pieces = (p.n + Elem<KIND>::kPer16 - 1) / Elem<KIND>::kPer16;
   if (pieces <= 64) return forward_launch<KIND, 1, 1>(p, block_dim, stream);
-  if (pieces <= 128) return forward_launch<KIND, 1, 2>(p, block_dim, stream);
+  if (pieces <= 128) return forward_launch<KIND, 2, 1>(p, block_dim, stream);
   if (pieces <= 256) return forward_launch<KIND, 4, 1>(p, block_dim, stream);
-  if (pieces <= 512) return forward_launch<KIND, 4, 2>(p, block_dim, stream);
-  if (pieces <= 1024) return forward_launch<KIND, 4, 4>(p, block_dim, stream);
+  if (pieces <= 512) return forward_launch<KIND, 8, 1>(p, block_dim, stream);
+  if (pieces <= 1024) return forward_launch<KIND, 16, 1>(p, block_dim, stream);
   if constexpr (kNormMaxColumns / Elem<KIND>::kPer16 > 2048)
     if (pieces > 2048) return forward_launch<KIND, 16, 4>(p, block_dim, stream);
   return forward_launch<KIND, 16, 2>(p, block_dim, stream);
@@ -238,9 +245,10 @@ inline Stretches plan_stretches(int64_t m, int64_t rows_per_gate, bool gate, int
 }
 
 template <int KIND, int WAVES, int ITEMS, bool kOneGate>
-__global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArgs p, Stretches s) {
+__global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGradArgs p, Stretches s) {
   constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64;
-  __shared__ float lds[2 * WAVES * 4];
+  constexpr bool kAhead = ITEMS == 1;
+  __shared__ __align__(16) float lds[2 * WAVES * 4];
   const int lane = threadIdx.x, wave = lane >> 6;
   const int64_t n = p.n;
   Piece<KIND, ITEMS> post, pre;
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
       row_sums<WAVES>(sums, lds, turn, wave);
       const float ry = rstd_of(sums[0], p.inv_n, p.eps), rf = rstd_of(sums[2], p.inv_n, p.eps);
       const float my = ry * sums[1] * p.inv_n;   // mean(a yn)
-      float t[ITEMS][V], vf[ITEMS][V], vg[ITEMS][V];
+      float t[ITEMS][V];
       float dot[1] = {0.f};
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
@@ -321,14 +329,14 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
           }
         }
         if (p.f) {
-          float vw[V];
-          Elem<KIND>::unpack(f.w[i], vf[i]);
+          float vf[V], vg[V], vw[V];
+          Elem<KIND>::unpack(f.w[i], vf);
           Elem<KIND>::unpack(post.w[i], vw);
-          if (p.gate) Elem<KIND>::unpack(gate.w[i], vg[i]);
+          if (p.gate) Elem<KIND>::unpack(gate.w[i], vg);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float gt = p.gate ? vg[i][j] * t[i][j] : t[i][j];
-            const float fn = vf[i][j] * rf;
+            const float gt = p.gate ? vg[j] * t[i][j] : t[i][j];
+            const float fn = vf[j] * rf;
             dot[0] += gt * vw[j] * fn;
             if constexpr (kOneGate) {
               acc_post[i][j] += t[i][j] * fn;
@@ -339,7 +347,10 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
           }
         }
       }
-      if (row + 1 < r1) fetch(row + 1);
+      // the next row is requested here, ahead of this row's stores and second round of sums; rows of
+      // several pieces per lane have no registers for two rows and request theirs when they are done
+      const Piece<KIND, ITEMS> f_here = f, gate_here = gate;
+      if (kAhead && row + 1 < r1) fetch(row + 1);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float o[V];
@@ -352,12 +363,14 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
         const float mf = dot[0] * p.inv_n;   // mean(b fn)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-          float o[V], vw[V];
+          float o[V], vf[V], vg[V], vw[V];
+          Elem<KIND>::unpack(f_here.w[i], vf);
           Elem<KIND>::unpack(post.w[i], vw);
+          if (p.gate) Elem<KIND>::unpack(gate_here.w[i], vg);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float b = (p.gate ? vg[i][j] * t[i][j] : t[i][j]) * vw[j];
-            o[j] = rf * (b - vf[i][j] * rf * mf);
+            const float b = (p.gate ? vg[j] * t[i][j] : t[i][j]) * vw[j];
+            o[j] = rf * (b - vf[j] * rf * mf);
           }
           store_item<KIND, kLanes>(p.df, row * p.ld_df, (int64_t)(lane + i * kLanes) * V, n, o);
         }
@@ -377,6 +390,7 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
           }
         }
       }
+      if (!kAhead && row + 1 < r1) fetch(row + 1);
     }
     float *const part_post = p.partial + stretch * n, *const part_pre = p.partial + (s.count + stretch) * n;
 #pragma unroll
@@ -393,35 +407,48 @@ __global__ __launch_bounds__(WAVES * 64) void norm_gate_backward(NormGateGradArg
 }
 
 // Adds the partial rows: blockIdx.y 0 gives dpre_weight, 1 dpost_weight, 2 + g gate row g (kOneGate
-// launches with a gate).  64 columns per workgroup, sixteen wavefronts share the rows.
-constexpr int kJoinWaves = 16;
+// launches with a gate).  64 columns per workgroup, four to a lane; 64 groups of lanes share the rows,
+// and their sums are added in order.
+constexpr int kJoinGroups = 64;
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
 template <int KIND>
-__global__ __launch_bounds__(kJoinWaves * 64) void norm_gate_join(NormGateGradArgs p, Stretches s, int64_t column_tiles) {
-  __shared__ float lds[kJoinWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(kJoinGroups * 16) void norm_gate_join(NormGateGradArgs p, Stretches s, int64_t column_tiles) {
+  __shared__ f32x4 lds[kJoinGroups][16];
+  const int four = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int what = blockIdx.y;
   if ((what == 0 && !p.dh) || (what == 1 && !p.f)) return;
   const float *const part = p.partial + (what == 0 ? s.count * p.n : 0);
   const int64_t first = what < 2 ? 0 : (what - 2) * s.per_span, last = what < 2 ? s.count : first + s.per_span;
   const bool weighted = what == 1 && s.one_gate && p.gate;
   for (int64_t tile = blockIdx.x; tile < column_tiles; tile += gridDim.x) {
-    const int64_t e = tile * 64 + lane;
-    float v = 0.f;
-    if (e < p.n) {
-      if (weighted) {
-        for (int64_t r = first + wave; r < last; r += kJoinWaves)
-          v += part[r * p.n + e] * Elem<KIND>::load(p.gate, r / s.per_span * p.ld_gate + e);
-      } else {
+    const int64_t e0 = tile * 64 + four * 4;
+    const int here = p.n - e0 < 4 ? (p.n > e0 ? (int)(p.n - e0) : 0) : 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int64_t r = first + wave; r < last; r += kJoinWaves) v += part[r * p.n + e];
-      }
-    }
-    lds[wave][lane] = v;
-    __syncthreads();
-    if (wave == 0 && e < p.n) {
-      float sum = 0.f;
+    for (int64_t r = first + group; r < last; r += kJoinGroups) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f}, w = {1.f, 1.f, 1.f, 1.f};
+      if (here == 4) {
+        x = *reinterpret_cast<const f32x4_u *>(part + r * p.n + e0);
+      } else {
 #pragma unroll
-      for (int w = 0; w < kJoinWaves; ++w) sum += lds[w][lane];
+        for (int j = 0; j < 3; ++j)
+          if (j < here) x[j] = part[r * p.n + e0 + j];
+      }
+      if (weighted) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < here) w[j] = Elem<KIND>::load(p.gate, r / s.per_span * p.ld_gate + e0 + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += x[j] * w[j];
+    }
+    lds[group][four] = v;
+    __syncthreads();
+    const int64_t e = tile * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && e < p.n) {
+      float sum = 0.f;
+#pragma unroll 8
+      for (int w = 0; w < kJoinGroups; ++w) sum += reinterpret_cast<const float *>(lds[w])[threadIdx.x];
       if (what == 0) Elem<KIND>::store(p.dpre_weight, e, sum);
       else if (what == 1) Elem<KIND>::store(p.dpost_weight, e, sum);
       else Elem<KIND>::store(p.dgate, (what - 2) * p.n + e, sum * Elem<KIND>::load(p.post_weight, e));
@@ -436,17 +463,13 @@ struct RowShape {
 };
 inline RowShape backward_shape(int64_t n, int elem_kind) {
   const int64_t pieces = elem_kind == kElemF32 ? (n + 3) / 4 : (n + 7) / 8;
-  if (pieces <= 64) return {1, 1};
-  if (pieces <= 128) return {1, 2};
-  if (pieces <= 256) return {4, 1};
-  if (pieces <= 512) return {4, 2};
-  if (pieces <= 1024) return {4, 4};
-  if (pieces <= 2048) return {8, 4};
-  return {16, 4};
+  for (int waves = 1; waves <= 16; waves *= 2)
+    if (pieces <= 64 * waves) return {waves, 1};
+  return {16, pieces <= 2048 ? 2 : 4};
 }
 inline Stretches backward_stretches(int64_t m, int64_t n, int64_t rows_per_gate, bool gate, int elem_kind) {
   const int waves = backward_shape(n, elem_kind).waves;
-  return plan_stretches(m, rows_per_gate, gate, (int64_t)device_cus() * (waves == 1 ? 8 : waves == 4 ? 2 : 1));
+  return plan_stretches(m, rows_per_gate, gate, (int64_t)device_cus() * (waves <= 8 ? 16 / waves : 1));
 }
 
 template <int KIND, int WAVES, int ITEMS>
@@ -464,7 +487,7 @@ LaunchStatus backward_launch(const NormGateGradArgs &p, const Stretches &s, uint
   const int64_t column_tiles = (p.n + 63) / 64;
   const int64_t gates = s.one_gate && p.f && p.gate ? (p.m + p.rows_per_gate - 1) / p.rows_per_gate : 0;
   AFIR_LAUNCH("norm_gate_join", (norm_gate_join<KIND>), dim3((unsigned)column_tiles, (unsigned)(2 + gates)),
-              dim3(kJoinWaves * 64), 0, stream, p, s, column_tiles);
+              dim3(kJoinGroups * 16), 0, stream, p, s, column_tiles);
   return after_launch();
 }
 
@@ -472,16 +495,16 @@ template <int KIND>
 LaunchStatus backward(const NormGateGradArgs &p, uint32_t block_dim, hipStream_t stream) {
   const Stretches s = backward_stretches(p.m, p.n, p.rows_per_gate, p.f && p.gate, KIND);
   const RowShape shape = backward_shape(p.n, KIND);
-  if (shape.waves == 1)
-    return shape.items == 1 ? backward_launch<KIND, 1, 1>(p, s, block_dim, stream)
-                            : backward_launch<KIND, 1, 2>(p, s, block_dim, stream);
-  if (shape.waves == 4)
-    return shape.items == 1   ? backward_launch<KIND, 4, 1>(p, s, block_dim, stream)
-           : shape.items == 2 ? backward_launch<KIND, 4, 2>(p, s, block_dim, stream)
-                              : backward_launch<KIND, 4, 4>(p, s, block_dim, stream);
   if constexpr (kNormMaxColumns / Elem<KIND>::kPer16 > 2048)
-    if (shape.waves == 16) return backward_launch<KIND, 16, 4>(p, s, block_dim, stream);
-  return backward_launch<KIND, 8, 4>(p, s, block_dim, stream);
+    if (shape.items == 4) return backward_launch<KIND, 16, 4>(p, s, block_dim, stream);
+  if (shape.items == 2) return backward_launch<KIND, 16, 2>(p, s, block_dim, stream);
+  switch (shape.waves) {
+    case 1: return backward_launch<KIND, 1, 1>(p, s, block_dim, stream);
+    case 2: return backward_launch<KIND, 2, 1>(p, s, block_dim, stream);
+    case 4: return backward_launch<KIND, 4, 1>(p, s, block_dim, stream);
+    case 8: return backward_launch<KIND, 8, 1>(p, s, block_dim, stream);
+    default: return backward_launch<KIND, 16, 1>(p, s, block_dim, stream);
+  }
 }
 
 }  // namespace

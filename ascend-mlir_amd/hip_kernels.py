@@ -261,39 +261,65 @@ def matmul_add_leakyrelu(a, b, bias, alpha=0.01, out=None, block_dim=0, stream=N
 #
 # Unlike the families above these take tensors of any of the three float types and rows
 # with a stride, launch on the device of their tensors, and check every tensor against the
-# others before they launch.
+# others before they launch.  They are called once per layer and token, so the checks are
+# one expression per tensor; only a tensor that fails it is looked at closely.
 
-_ELEM_TYPES = None
+_ELEM_TYPES = {}
+_entries = {}
 
 
 def _elem_type(dtype, what):
-    global _ELEM_TYPES
-    if _ELEM_TYPES is None:
+    if not _ELEM_TYPES:
         import torch
-        _ELEM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        _ELEM_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     code = _ELEM_TYPES.get(dtype)
     if code is None:
         raise AfirHipError(f"{what}: expected float32, float16 or bfloat16, got {dtype}")
     return code
 
 
-def _on(t, device, what):
-    """A tensor on the device that the call's first tensor is on."""
+def _device_of(t, what):
+    """Index of the device of a call's first tensor."""
+    try:
+        index = t.get_device()
+    except AttributeError:
+        index = -1
+    if index < 0:
+        raise AfirHipError(f"{what}: expected a device tensor")
+    return index
+
+
+def _explain(t, shape, dtype, index, what):
+    """Raises for the first thing about t that is not as it has to be."""
     import torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise AfirHipError(f"{what}: expected a device tensor")
-    if device is not None and t.device != device:
-        raise AfirHipError(f"{what}: on {t.device}, the call's first tensor is on {device}")
-    return t
-
-
-def _rows(t, shape, dtype, device, what):
-    """A matrix of rows that may have a stride; returns the stride in elements."""
-    _on(t, device, what)
+    if t.get_device() != index:
+        raise AfirHipError(f"{what}: on {t.device}, the call's first tensor is on device {index}")
     if t.dtype != dtype:
         raise AfirHipError(f"{what}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise AfirHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _dense(t, shape, dtype, index, what):
+    try:
+        if t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.get_device() == index:
+            return
+    except AttributeError:
+        pass
+    _explain(t, shape, dtype, index, what)
+    raise AfirHipError(f"{what}: expected a contiguous tensor")
+
+
+def _rows(t, shape, dtype, index, what):
+    """A matrix of rows that may have a stride; returns the stride in elements."""
+    try:
+        if t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.get_device() == index:
+            return shape[1]
+    except AttributeError:
+        pass
+    _explain(t, shape, dtype, index, what)
     ld, unit = t.stride()
     if unit != 1 and shape[1] > 1:
         raise AfirHipError(f"{what}: the numbers of a row must be adjacent")
@@ -304,46 +330,43 @@ def _rows(t, shape, dtype, device, what):
     return ld
 
 
-def _dense(t, shape, dtype, device, what):
-    _on(t, device, what)
-    if t.dtype != dtype:
-        raise AfirHipError(f"{what}: expected {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise AfirHipError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise AfirHipError(f"{what}: expected a contiguous tensor")
-    return t
-
-
-def _launch_on(device, symbol, block_dim, stream, tensors, workspace, tiling):
-    """Launch with `device` current; tensors may be None.  The stream is the caller's or
-    the current one of that device."""
+def _launch_on(index, symbol, block_dim, stream, tiling, workspace, *tensors):
+    """Launch with device `index` current; tensors may be None.  The stream is the caller's
+    or the current one of that device."""
     import torch
-    L = load()
+    fn = _entries.get(symbol)
+    if fn is None:
+        fn = _entries[symbol] = getattr(load(), symbol)
     ptrs = [None if t is None else t.data_ptr() for t in tensors]
-    ws = None if workspace is None else workspace.data_ptr()
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            st = stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
-            rc = getattr(L, symbol)(block_dim, st, *ptrs, ws, tiling)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            st = torch.cuda.current_stream(index).cuda_stream if stream is None else stream
+            rc = fn(block_dim, st, *ptrs, workspace, tiling)
     else:
-        st = stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
-        rc = getattr(L, symbol)(block_dim, st, *ptrs, ws, tiling)
+        # (the raw handle: building a Stream object takes as long as the rest of the call)
+        st = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream
+        rc = fn(block_dim, st, *ptrs, workspace, tiling)
     if rc:
         _check(rc)
 
 
-def _workspace(query, tiling, device, stream):
+def _workspace(query, tiling, like, stream):
     """Scratch of the size that the library asks for, from torch's allocator, which hands it
     out again only to work that follows on the stream of this call."""
     import torch
-    size = getattr(load(), query)(tiling)
+    fn = _entries.get(query)
+    if fn is None:
+        fn = _entries[query] = getattr(load(), query)
+    size = fn(tiling)
     if not size:
         return None
-    ws = torch.empty((size,), dtype=torch.uint8, device=device)
+    ws = torch.empty((size,), dtype=torch.uint8, device=like.device)
     if stream is not None:
-        ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
     return ws
+
+
+_PACK5, _PACK11, _PACK13 = (struct.Struct(f"<{count}q").pack for count in (5, 11, 13))
 
 
 def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_values=False,
@@ -356,30 +379,30 @@ def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_valu
     return_values (or values=) also the numbers they stand for, in x's shape and type.
     Blocks that hold an infinity or a NaN read as NaN throughout."""
     import torch
-    _on(x, None, "x")
+    index = _device_of(x, "x")
     if x.dim() != 2:
         raise AfirHipError("mxfp4_quantize: x must have two dimensions")
     if axis not in (-1, 0, 1):
         raise AfirHipError("mxfp4_quantize: axis must be 0 or 1 (or -1)")
-    kind = _elem_type(x.dtype, "x")
-    ld = _rows(x, x.shape, x.dtype, None, "x")
-    k, r = x.shape if axis == 0 else (x.shape[1], x.shape[0])
+    shape, dtype = x.shape, x.dtype
+    kind = _elem_type(dtype, "x")
+    ld = _rows(x, shape, dtype, index, "x")
+    k, r = shape if axis == 0 else (shape[1], shape[0])
     kb = (k + 31) // 32
-    dev = x.device
     if codes is None:
-        codes = torch.empty((r, kb * 16), dtype=torch.uint8, device=dev)
+        codes = torch.empty((r, kb * 16), dtype=torch.uint8, device=x.device)
     else:
-        _dense(codes, (r, kb * 16), torch.uint8, dev, "codes")
+        _dense(codes, (r, kb * 16), torch.uint8, index, "codes")
     if scales is None:
-        scales = torch.empty((r, kb), dtype=torch.float8_e8m0fnu, device=dev)
+        scales = torch.empty((r, kb), dtype=torch.float8_e8m0fnu, device=x.device)
     else:
-        _dense(scales, (r, kb), torch.float8_e8m0fnu, dev, "scales")
+        _dense(scales, (r, kb), torch.float8_e8m0fnu, index, "scales")
     if values is not None:
-        _dense(values, x.shape, x.dtype, dev, "values")
+        _dense(values, shape, dtype, index, "values")
     elif return_values:
-        values = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    _launch_on(dev, "afir_hip_launch_mxfp4_quantize", block_dim, stream, (x, codes, scales, values), None,
-               struct.pack("<5q", x.shape[0], x.shape[1], ld, 0 if axis == 0 else 1, kind))
+        values = torch.empty(shape, dtype=dtype, device=x.device)
+    _launch_on(index, "afir_hip_launch_mxfp4_quantize", block_dim, stream,
+               _PACK5(shape[0], shape[1], ld, 0 if axis == 0 else 1, kind), None, x, codes, scales, values)
     return (codes, scales) if values is None else (codes, scales, values)
 
 
@@ -390,40 +413,45 @@ def mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias=None, alpha=0.01, 
     out is given) is the type of bias and out.  k: K itself, where it is not a multiple of
     32 (only checked against the codes)."""
     import torch
-    _on(a, None, "a")
-    dev = a.device
-    if a.dim() != 2 or b.dim() != 2:
-        raise AfirHipError("mxfp4_matmul_add_leakyrelu: codes must have two dimensions")
-    m, n, kb = a.shape[0], b.shape[0], a.shape[1] // 16
-    if a.shape[1] % 16:
+    index = _device_of(a, "a")
+    try:
+        (m, row), (n, _) = a.shape, b.shape
+    except (AttributeError, ValueError):
+        raise AfirHipError("mxfp4_matmul_add_leakyrelu: codes must be tensors of two dimensions") from None
+    kb = row // 16
+    if row % 16:
         raise AfirHipError("mxfp4_matmul_add_leakyrelu: code rows must be whole blocks of 16 bytes")
     if k is None:
         k = kb * 32
     elif (k + 31) // 32 != kb:
         raise AfirHipError(f"mxfp4_matmul_add_leakyrelu: k = {k} does not have {kb} blocks")
-    _dense(a, (m, kb * 16), torch.uint8, dev, "a")
-    _dense(b, (n, kb * 16), torch.uint8, dev, "b")
-    _dense(a_scales, (m, kb), torch.float8_e8m0fnu, dev, "a_scales")
-    _dense(b_scales, (n, kb), torch.float8_e8m0fnu, dev, "b_scales")
+    _dense(a, (m, row), torch.uint8, index, "a")
+    _dense(b, (n, row), torch.uint8, index, "b")
+    _dense(a_scales, (m, kb), torch.float8_e8m0fnu, index, "a_scales")
+    _dense(b_scales, (n, kb), torch.float8_e8m0fnu, index, "b_scales")
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=dev)
+        dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        kind = _elem_type(dtype, "out")
+        out = torch.empty((m, n), dtype=dtype, device=a.device)
     else:
-        _dense(out, (m, n), out.dtype if out_dtype is None else out_dtype, dev, "out")
-    kind = _elem_type(out.dtype, "out")
+        dtype = out.dtype if out_dtype is None else out_dtype
+        kind = _elem_type(dtype, "out")
+        _dense(out, (m, n), dtype, index, "out")
     if bias is not None:
-        _dense(bias, (n,), out.dtype, dev, "bias")
-    tiling = struct.pack("<5q", m, k, n, f32_bits(alpha), kind)
-    ws = _workspace("afir_hip_mxfp4_matmul_workspace_bytes", tiling, dev, stream)
-    _launch_on(dev, "afir_hip_launch_mxfp4_matmul_add_leakyrelu", block_dim, stream,
-               (a, a_scales, b, b_scales, bias, out), ws, tiling)
+        _dense(bias, (n,), dtype, index, "bias")
+    tiling = _PACK5(m, k, n, f32_bits(alpha), kind)
+    ws = _workspace("afir_hip_mxfp4_matmul_workspace_bytes", tiling, a, stream)
+    _launch_on(index, "afir_hip_launch_mxfp4_matmul_add_leakyrelu", block_dim, stream, tiling,
+               None if ws is None else ws.data_ptr(), a, a_scales, b, b_scales, bias, out)
     return out
 
 
-def _gate_rows(gate, m, n, rows_per_gate, dtype, dev):
+def _gate_rows(gate, m, n, rows_per_gate, dtype, index):
     """(rows_per_gate, row stride) of a gate [G, N] or [N] for m rows."""
     if gate is None:
         return max(m, 1), n
-    _on(gate, dev, "gate")
+    if _device_of(gate, "gate") != index:
+        _explain(gate, None, None, index, "gate")
     if gate.dim() == 1:
         gate = gate.unsqueeze(0)
     if gate.dim() != 2:
@@ -433,7 +461,7 @@ def _gate_rows(gate, m, n, rows_per_gate, dtype, dev):
         rows_per_gate = max(m, 1) if g == 1 else 1
     if rows_per_gate < 1 or -(-m // rows_per_gate) != g:
         raise AfirHipError(f"gate: {g} rows of {rows_per_gate} do not cover {m} rows")
-    return rows_per_gate, _rows(gate, (g, n), dtype, dev, "gate")
+    return rows_per_gate, _rows(gate, (g, n), dtype, index, "gate")
 
 
 def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, residual_scale=1.0, eps=1e-6,
@@ -447,36 +475,35 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
     (the norm ahead of the first block); without pre_weight there is no h.  Returns (y, h).
     y=x and h=f work in place."""
     import torch
-    _on(x, None, "x")
+    index = _device_of(x, "x")
     if x.dim() != 2:
         raise AfirHipError("norm_gate_residual: x must have two dimensions")
-    dev, dtype = x.device, x.dtype
+    dtype = x.dtype
     kind = _elem_type(dtype, "x")
     m, n = shape = x.shape
-    ld_x = _rows(x, shape, dtype, None, "x")
+    ld_x = _rows(x, shape, dtype, index, "x")
     ld_f = ld_gate = ld_y = ld_h = n
     if f is None:
         if post_weight is not None or gate is not None or y is not None or pre_weight is None:
             raise AfirHipError("norm_gate_residual: without f only x and pre_weight are used")
         rows_per_gate = max(m, 1)
     else:
-        ld_f = _rows(f, shape, dtype, dev, "f")
-        _dense(post_weight, (n,), dtype, dev, "post_weight")
-        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, dev)
+        ld_f = _rows(f, shape, dtype, index, "f")
+        _dense(post_weight, (n,), dtype, index, "post_weight")
+        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, index)
         if y is None:
-            y = torch.empty(shape, dtype=dtype, device=dev)
-        ld_y = _rows(y, shape, dtype, dev, "y")
+            y = torch.empty(shape, dtype=dtype, device=x.device)
+        ld_y = _rows(y, shape, dtype, index, "y")
     if pre_weight is not None:
-        _dense(pre_weight, (n,), dtype, dev, "pre_weight")
+        _dense(pre_weight, (n,), dtype, index, "pre_weight")
         if h is None:
-            h = torch.empty(shape, dtype=dtype, device=dev)
-        ld_h = _rows(h, shape, dtype, dev, "h")
+            h = torch.empty(shape, dtype=dtype, device=x.device)
+        ld_h = _rows(h, shape, dtype, index, "h")
     elif h is not None:
         raise AfirHipError("norm_gate_residual: h needs pre_weight")
-    _launch_on(dev, "afir_hip_launch_norm_gate_residual", block_dim, stream,
-               (x, f, post_weight, gate, pre_weight, y, h), None,
-               struct.pack("<11q", m, n, rows_per_gate, ld_x, ld_f, ld_gate, ld_y, ld_h, f32_bits(residual_scale),
-                           f32_bits(eps), kind))
+    _launch_on(index, "afir_hip_launch_norm_gate_residual", block_dim, stream,
+               _PACK11(m, n, rows_per_gate, ld_x, ld_f, ld_gate, ld_y, ld_h, f32_bits(residual_scale), f32_bits(eps), kind),
+               None, x, f, post_weight, gate, pre_weight, y, h)
     return (x if f is None else y), h
 
 
@@ -486,7 +513,7 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     those of its results and the y it returned; None where it had no such input.  dy None:
     zero.  dh, pre_weight None: the call had no h (y is not read then)."""
     import torch
-    _on(y, None, "y")
+    index = _device_of(y, "y")
     if y.dim() != 2:
         raise AfirHipError("norm_gate_residual_backward: y must have two dimensions")
     dev, dtype = y.device, y.dtype
@@ -494,7 +521,7 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     m, n = shape = y.shape
     if m == 0 or n == 0:
         raise AfirHipError("norm_gate_residual_backward: empty tensors have no gradients to write")
-    ld_y = _rows(y, shape, dtype, None, "y")
+    ld_y = _rows(y, shape, dtype, index, "y")
     ld_dy = ld_dh = ld_f = ld_gate = n
     if (dh is None) != (pre_weight is None):
         raise AfirHipError("norm_gate_residual_backward: dh and pre_weight go together")
@@ -503,30 +530,30 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     if dh is None and f is None:
         raise AfirHipError("norm_gate_residual_backward: f or dh is needed")
     if dy is not None:
-        ld_dy = _rows(dy, shape, dtype, dev, "dy")
+        ld_dy = _rows(dy, shape, dtype, index, "dy")
     df = dpost = dgate = dpre = None
     if dh is not None:
-        ld_dh = _rows(dh, shape, dtype, dev, "dh")
-        _dense(pre_weight, (n,), dtype, dev, "pre_weight")
+        ld_dh = _rows(dh, shape, dtype, index, "dh")
+        _dense(pre_weight, (n,), dtype, index, "pre_weight")
         dpre = torch.empty((n,), dtype=dtype, device=dev)
     if f is None:
         if post_weight is not None or gate is not None:
             raise AfirHipError("norm_gate_residual_backward: post_weight and gate need f")
         rows_per_gate = m
     else:
-        ld_f = _rows(f, shape, dtype, dev, "f")
-        _dense(post_weight, (n,), dtype, dev, "post_weight")
-        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, dev)
+        ld_f = _rows(f, shape, dtype, index, "f")
+        _dense(post_weight, (n,), dtype, index, "post_weight")
+        rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, index)
         df = torch.empty(shape, dtype=dtype, device=dev)
         dpost = torch.empty((n,), dtype=dtype, device=dev)
         if gate is not None:
             dgate = torch.empty(gate.shape, dtype=dtype, device=dev)
     dx = torch.empty(shape, dtype=dtype, device=dev)
-    tiling = struct.pack("<13q", m, n, rows_per_gate, ld_dy, ld_dh, ld_y, ld_f, ld_gate, n, n,
-                         f32_bits(residual_scale), f32_bits(eps), kind)
-    ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, dev, stream)
-    _launch_on(dev, "afir_hip_launch_norm_gate_residual_backward", block_dim, stream,
-               (dy, dh, None if dh is None else y, f, post_weight, gate, pre_weight, dx, df, dpost, dgate, dpre), ws, tiling)
+    tiling = _PACK13(m, n, rows_per_gate, ld_dy, ld_dh, ld_y, ld_f, ld_gate, n, n,
+                     f32_bits(residual_scale), f32_bits(eps), kind)
+    ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, y, stream)
+    _launch_on(index, "afir_hip_launch_norm_gate_residual_backward", block_dim, stream, tiling, ws.data_ptr(),
+               dy, dh, None if dh is None else y, f, post_weight, gate, pre_weight, dx, df, dpost, dgate, dpre)
     return dx, df, dpost, dgate, dpre
 
 
