@@ -47,6 +47,7 @@ KERNEL_SOURCES = [
     ("kernels/mxfp4_quantize.hip", []),
     ("kernels/mxfp4_matmul.hip", []),
     ("kernels/mxfp4_matmul_dma.hip", []),
+    ("kernels/mxfp4_matmul_ring.hip", []),
     ("kernels/norm_gate.hip", []),
     ("kernels/region.hip", STRICT),
     ("target/region_program.cpp", []),

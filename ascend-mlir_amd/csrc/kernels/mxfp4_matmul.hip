@@ -16,15 +16,17 @@ __device__ __forceinline__ void finish_one(const MxOperands &p, int m, int n, fl
   Elem<KIND>::store(p.out, (int64_t)m * p.n + n, v);
 }
 
-// Few rows of A (MT tiles of 16): the time is that of reading B.  A workgroup owns 16 * NT
-// columns and its eight wavefronts deal the blocks of K out among themselves, 16 blocks (256 bytes
-// of a row) at a step.  Of a step, lane group g of a wavefront takes blocks g, 4 + g, 8 + g and
-// 12 + g: each of the four loads then covers 64 adjacent bytes of each of the 16 rows, a quarter of
-// the segments that four adjacent blocks per lane would touch (that was the bound: 48 rows of A
-// 15.9 us, one row 9.1).  The row's sixteen scales come as one 16-byte load and are shifted to the
-// lane's byte.  Everything of a step is requested before the first product, where the registers
-// allow it (kAhead) the next step's too.  The eight partial sums meet in LDS and are added in a
-// fixed order.
+// Up to 16 rows of A: the time is that of reading B.  A workgroup owns 16 * NT columns and its eight
+// wavefronts deal the blocks of K out among themselves, 16 blocks (256 bytes of a row) at a step.  Of a
+// step, lane group g of a wavefront takes blocks g, 4 + g, 8 + g and 12 + g: each of the four loads then
+// covers 64 adjacent bytes of each of the 16 rows, a quarter of the segments that four adjacent blocks per
+// lane would touch.  The row's sixteen scales come as one 16-byte load and are shifted to the lane's byte.
+// Everything of a step is requested before the first product; two workgroups on a compute unit cover the
+// rest (requesting the next step ahead as well gained nothing: 9.3 against 9.0 us for one row at
+// 8192 x 8192).  The eight partial sums meet in LDS and are added in a fixed order.
+// One row: 9.0 us at 8192 x 8192 (4.0 TB/s; the bytes alone take 7.3 as a large copy moves them), 3.5 at
+// 4096 x 4096; 16 rows at 8192 x 8192 9.7.
+// Also products with K below 256 (MT = 4 above 16 rows).
 constexpr int kRowsWaves = 8;
 
 // 16 rows' codes and scales of one step
@@ -51,10 +53,9 @@ struct RowsPiece {
 };
 
 template <int MT, int NT, int KIND>
-__global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands p, int tiles_n, int chunks_m,
-                                                                     int blocks) {
+__global__ __launch_bounds__(kRowsWaves * 64, MT == 1 ? 4 : 2) void mxfp4_matmul_rows(MxOperands p, int tiles_n,
+                                                                                      int chunks_m, int blocks) {
   constexpr int kCols = 16 * NT, kRows = 16 * MT;
-  constexpr bool kAhead = MT + NT <= 4;
   __shared__ f32x4 part[kRowsWaves][kRows * kCols / 4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, g = lane >> 4;
   const int shift = 8 * g;
@@ -75,13 +76,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands 
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    RowsPiece a[MT], b[NT], a_next[kAhead ? MT : 1], b_next[kAhead ? NT : 1];
-    auto fetch = [&](int step, RowsPiece *pa, RowsPiece *pb) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) pb[j].load(p.b, p.b_scales, row_b[j], p.kb, step, g);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) pa[i].load(p.a, p.a_scales, row_a[i], p.kb, step, g);
-    };
+    RowsPiece a[MT], b[NT];
     auto multiply = [&]() {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -98,21 +93,12 @@ __global__ __launch_bounds__(kRowsWaves * 64) void mxfp4_matmul_rows(MxOperands 
     };
     const int whole = p.kb / 16;   // steps of 16 blocks
     int step = wave;
-    if constexpr (kAhead) {
-      if (step < whole) fetch(step, a, b);
-      for (; step < whole; step += kRowsWaves) {
-        if (step + kRowsWaves < whole) fetch(step + kRowsWaves, a_next, b_next);
-        multiply();
+    for (; step < whole; step += kRowsWaves) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) a[i] = a_next[i];
+      for (int j = 0; j < NT; ++j) b[j].load(p.b, p.b_scales, row_b[j], p.kb, step, g);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b[j] = b_next[j];
-      }
-    } else {
-      for (; step < whole; step += kRowsWaves) {
-        fetch(step, a, b);
-        multiply();
-      }
+      for (int i = 0; i < MT; ++i) a[i].load(p.a, p.a_scales, row_a[i], p.kb, step, g);
+      multiply();
     }
     if (step == whole && whole * 16 < p.kb) {
 #pragma unroll
@@ -150,12 +136,23 @@ LaunchStatus rows_launch(const MxOperands &p, uint32_t block_dim, hipStream_t st
   return after_launch();
 }
 
+// A tile per workgroup up to 64 rows (9.2 us against 15.8 on the kernel above at 48 x 8200 x 4096), and while
+// each compute unit gets at most one of 128 x 128 (512 x 8192 x 8192: 27 us, 28 on tiles in turn); beyond that
+// tiles in turn (1024 x 8192 x 8192: 45 us against 55).
+bool one_tile_each(const MxOperands &p) {
+  return p.m > 16 && mxfp4_ring_supported(p) &&
+         (p.m <= 64 || (int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128) <= device_cus());
+}
+
 template <int KIND>
 LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hipStream_t stream) {
-  if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
+  // Up to 16 rows; 16 columns a workgroup where that gives no compute unit a second one (4096 x 4096, one row:
+  // 3.5 us against 4.8 with 32; 8192 x 8192, 16 rows: 11.8 against 9.7).
+  if (p.m <= 16 && p.n <= 16 * device_cus()) return rows_launch<1, 1, KIND>(p, block_dim, stream);
   if (p.m <= 16) return rows_launch<1, 2, KIND>(p, block_dim, stream);
-  if (p.m <= 32) return rows_launch<2, 2, KIND>(p, block_dim, stream);
-  if (p.m <= 48) return rows_launch<3, 2, KIND>(p, block_dim, stream);
+  if (one_tile_each(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
+  if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
+  if (mxfp4_ring_supported(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
   return rows_launch<4, 2, KIND>(p, block_dim, stream);
 }
 
@@ -168,7 +165,7 @@ size_t mxfp4_matmul_workspace(int64_t m, int64_t k, int64_t n) {
   p.m = (int)m;
   p.n = (int)n;
   p.kb = kb;
-  return mxfp4_dma_supported(p) ? mxfp4_dma_workspace(m, kb, n) : 0;
+  return mxfp4_dma_supported(p) && !one_tile_each(p) ? mxfp4_dma_workspace(m, kb, n) : 0;
 }
 
 LaunchStatus launch_mxfp4_matmul(const void *a, const void *a_scales, const void *b, const void *b_scales,

@@ -1,4 +1,4 @@
-// MXFP4 products of more than a few rows: tiles in LDS, the matrix cores fed from there.
+// MXFP4 products of more output tiles than compute units: tiles in LDS, the matrix cores fed from there.
 //
 // A K slice is 256 numbers: one 128-byte line of every row of A and B.  Lines are copied global ->
 // LDS directly (global_load_lds, 16 bytes per lane, no registers in between) into two slots each;
@@ -13,8 +13,12 @@
 // the upper half of A from the fourth: a line has a slice and a half to arrive, and a barrier
 // every two phases says both that what comes next has landed and that what goes next has been
 // read.  The refills walk ahead of the products across tile boundaries, so nothing drains between
-// the tiles of a workgroup; only the output passes in between.  Every operand read and every load sits behind a matrix instruction (pinned with
-// scheduling barriers), as in matmul_dma_kernel.h.
+// the tiles of a workgroup; only the output passes in between.  Every operand read and every load sits
+// behind a matrix instruction (pinned with scheduling barriers), as in matmul_dma_kernel.h.
+//
+// 8192 x 8192 x 8192 into bfloat16: 232 us, 4.7 PFLOP/s, 6 us of it the arranging of the scales.  With
+// operands that are all alike it is 176 us (6.2 PFLOP/s): what bounds random ones is the power that the
+// matrix cores draw (fed from registers alone they reach 7.4 PFLOP/s, 9.6 with constant operands).
 //
 // Rows past the end of A or B repeat the last row.  A last slice that is not whole starts early, so
 // that it ends with the row; the scales that go with the blocks it repeats are 2^-127 on both sides,
@@ -24,61 +28,11 @@
 // bytes a lane needs of each of four 16-row tiles are adjacent: a wave reads its 128 x 8 scales of
 // a slice with two 8-byte LDS reads, and they come into LDS with two small loads per wave.  Read as
 // they are stored it would take twelve 2-byte reads.
-#include <type_traits>
-
 #include "mxfp4_mfma.h"
 
 namespace afir {
 
 namespace {
-
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-template <int OFF>
-__device__ __forceinline__ void read16(uint32_t addr, u32x4 &dst) {
-  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(dst) : "v"(addr), "n"(OFF) : "memory");
-}
-template <int OFF>
-__device__ __forceinline__ void read8(uint32_t addr, u32x2 &dst) {
-  asm volatile("ds_read_b64 %0, %1 offset:%2" : "=&v"(dst) : "v"(addr), "n"(OFF) : "memory");
-}
-// The lane number, opaque to the compiler: what is computed from it is computed where it stands, once
-// per tile, and not kept in registers (or scratch memory, whose accesses would wait for every load in
-// flight) through the slices.
-__device__ __forceinline__ int lane_here() {
-  int lane;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
-  return lane;
-}
-// lanes 16 .. 31 and 48 .. 63 of `a` and lanes 0 .. 15 and 32 .. 47 of `b` change places
-__device__ __forceinline__ u32x2 swap_odd_even(uint32_t a, uint32_t b) {
-  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-  return u32x2{(uint32_t)r[0], (uint32_t)r[1]};
-}
-// of every 16 lanes: x in lanes 0 .. 7, y of those lanes in lanes 8 .. 15
-__device__ __forceinline__ uint32_t exchange_high(uint32_t x, uint32_t y) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)y, 0x128, 0xf, 0xc, false);   // row_ror:8, lanes 8 .. 15
-}
-// ... x of lanes 8 .. 15 in lanes 0 .. 7, y in lanes 8 .. 15
-__device__ __forceinline__ uint32_t exchange_low(uint32_t x, uint32_t y) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)y, (int)x, 0x128, 0xf, 0x3, false);   // row_ror:8, lanes 0 .. 7
-}
-template <int I, int N, typename F>
-__device__ __forceinline__ void static_for(F &&f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>{});
-    static_for<I + 1, N>(f);
-  }
-}
-// registers that reads in flight were given, handed back as fresh values after the wait
-template <typename T, int N>
-__device__ __forceinline__ void settle(T (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
-}
 
 // item R of N goes behind matrix instruction place(R, N, NM) of NM; reads (the first `reads`) one after
 // the other, loads two instructions apart where there is room
@@ -86,21 +40,19 @@ constexpr int place(int r, int n, int nm, int reads) {
   return n > nm ? r * nm / n : r < reads || reads + 2 * (n - reads) > nm ? r : reads + 2 * (r - reads);
 }
 
-constexpr int kSliceBytes = 128;          // of a row: 256 codes, 8 blocks
-constexpr int kSliceBlocks = 8;
 constexpr int kUnitRows = 64;             // rows whose scales of a slice are one piece of 512 bytes
-constexpr int kUnitBytes = kUnitRows * kSliceBlocks;
+constexpr int kUnitBytes = kUnitRows * kMxSliceBlocks;
 constexpr int kUnitPad = 4;               // units are allotted in fours: the rows of the largest tile
 
 inline int64_t scale_units(int64_t rows) {
   return (rows + kUnitRows * kUnitPad - 1) / (kUnitRows * kUnitPad) * kUnitPad;
 }
-inline int64_t slices_of(int64_t kb) { return (kb + kSliceBlocks - 1) / kSliceBlocks; }
+inline int64_t slices_of(int64_t kb) { return (kb + kMxSliceBlocks - 1) / kMxSliceBlocks; }
 
 // scales [rows][kb] -> [slice][unit][lane][4 tiles][2]: lane l = 16 g + r holds, of row 16 i + r of the
 // unit, blocks g and 4 + g of the slice.  A's units first, then B's.  A workgroup turns a unit's rows
 // of 16 slices (128 bytes each) in LDS, so that both sides move whole lines.
-constexpr int kTurnSlices = 16, kTurnPitch = kTurnSlices * kSliceBlocks + 4;
+constexpr int kTurnSlices = 16, kTurnPitch = kTurnSlices * kMxSliceBlocks + 4;
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 __global__ __launch_bounds__(256) void mxfp4_arrange_scales(MxOperands p, int units_a, int units_b, int slices,
                                                             int turns, unsigned char *__restrict__ out) {
@@ -112,7 +64,7 @@ __global__ __launch_bounds__(256) void mxfp4_arrange_scales(MxOperands p, int un
     const int unit = is_a ? unit_all : unit_all - units_a, units = is_a ? units_a : units_b, rows = is_a ? p.m : p.n;
     const uint8_t *const s = is_a ? p.a_scales : p.b_scales;
     for (int i = threadIdx.x; i < kUnitRows * 8; i += 256) {
-      const int r = i >> 3, at = (i & 7) * 16, block = s0 * kSliceBlocks + at;
+      const int r = i >> 3, at = (i & 7) * 16, block = s0 * kMxSliceBlocks + at;
       const int row = unit * kUnitRows + r < rows ? unit * kUnitRows + r : rows - 1;
       const uint8_t *const q = s + (int64_t)row * p.kb + block;
       uint32_t w[4] = {0, 0, 0, 0};   // past the end: 2^-127
@@ -134,8 +86,8 @@ __global__ __launch_bounds__(256) void mxfp4_arrange_scales(MxOperands p, int un
       const int lane = i & 63, ds = i >> 6, slice = s0 + ds, g = lane >> 4;
       if (slice < slices) {
         // a last slice that starts `early` blocks early: those get 2^-127
-        const int early = (slice + 1) * kSliceBlocks > p.kb ? (slice + 1) * kSliceBlocks - p.kb : 0;
-        const unsigned char *const from = tile + (lane & 15) * kTurnPitch + ds * kSliceBlocks + g - early;
+        const int early = (slice + 1) * kMxSliceBlocks > p.kb ? (slice + 1) * kMxSliceBlocks - p.kb : 0;
+        const unsigned char *const from = tile + (lane & 15) * kTurnPitch + ds * kMxSliceBlocks + g - early;
         uint32_t w[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -148,25 +100,12 @@ __global__ __launch_bounds__(256) void mxfp4_arrange_scales(MxOperands p, int un
   }
 }
 
-__device__ __forceinline__ void map_tile(int p, int tiles_m, int tiles_n, int &tm, int &tn) {
-  // tiles of one XCD (workgroup i runs on XCD i % 8) form patches of four tile rows
-  const int ntiles = tiles_m * tiles_n;
-  int q = p;
-  if (ntiles % kNumXCD == 0) q = (p % kNumXCD) * (ntiles / kNumXCD) + p / kNumXCD;
-  constexpr int kGroupM = 4;
-  const int per_group = kGroupM * tiles_n;
-  const int group = q / per_group, within = q % per_group, first_m = group * kGroupM;
-  const int gsize = tiles_m - first_m < kGroupM ? tiles_m - first_m : kGroupM;
-  tm = first_m + within % gsize;
-  tn = within / gsize;
-}
-
 // WM x WN wavefronts, each TM x TN tiles of 16 x 16.
 template <int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kBM = WM * TM * 16, kBN = WN * TN * 16;
-  static constexpr int kSlotA = kBM * kSliceBytes, kSlotB = kBN * kSliceBytes;
-  static constexpr int kScaleA = kBM * kSliceBlocks, kScale = kScaleA + kBN * kSliceBlocks;   // A's units, then B's
+  static constexpr int kSlotA = kBM * kMxSliceBytes, kSlotB = kBN * kMxSliceBytes;
+  static constexpr int kScaleA = kBM * kMxSliceBlocks, kScale = kScaleA + kBN * kMxSliceBlocks;   // A's units, then B's
   static constexpr int kOffB = 2 * kSlotA, kOffScale = kOffB + 2 * kSlotB;
   static constexpr int kLds = kOffScale + 2 * kScale;
   static constexpr int kHalf = TM / 2;
@@ -196,8 +135,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
 
   // ---- operand reads: lane l reads row l % 16 of a tile, chunk l / 16 + 4 step ----
   const uint32_t swz = (uint32_t)((li >> 1) & 7);
-  const uint32_t rd_a0 = (uint32_t)((wm * TM * 16 + li) * kSliceBytes) + (g ^ swz) * 16;   // step 1: ^ 64
-  const uint32_t rd_b0 = (uint32_t)(T::kOffB + (wn * TN * 16 + li) * kSliceBytes) + (g ^ swz) * 16;
+  const uint32_t rd_a0 = (uint32_t)((wm * TM * 16 + li) * kMxSliceBytes) + (g ^ swz) * 16;   // step 1: ^ 64
+  const uint32_t rd_b0 = (uint32_t)(T::kOffB + (wn * TN * 16 + li) * kMxSliceBytes) + (g ^ swz) * 16;
   const uint32_t rd_sa = (uint32_t)(T::kOffScale + wm * (TM / 4) * kUnitBytes + lane * 8);
   const uint32_t rd_sb = (uint32_t)(T::kOffScale + T::kScaleA + wn * (TN / 4) * kUnitBytes + lane * 8);
 
@@ -224,8 +163,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
   auto set_slice = [&]() {
     // the last slice of a row that is no whole number of them starts early enough to end with the row;
     // the blocks it has in common with the one before it come with scales that take them out
-    const uint32_t at = (uint32_t)cur_slice * kSliceBytes;
-    const uint32_t column = at < pitch - kSliceBytes ? at : pitch - kSliceBytes;
+    const uint32_t at = (uint32_t)cur_slice * kMxSliceBytes;
+    const uint32_t column = at < pitch - kMxSliceBytes ? at : pitch - kMxSliceBytes;
     at_a = base_a + column;
     at_b = base_b + column;
     at_s = base_s + (int64_t)cur_slice * scale_step;
@@ -236,8 +175,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
     const int m0 = tm * T::kBM, n0 = tn * T::kBN;
     base_a = p.a + (int64_t)m0 * pitch;
     base_b = p.b + (int64_t)n0 * pitch;
-    base_s = scales + (scales_of_a ? (int64_t)m0 * kSliceBlocks + wave * T::kScaleShare
-                                   : ((int64_t)units_a * slices * kUnitRows + n0) * kSliceBlocks +
+    base_s = scales + (scales_of_a ? (int64_t)m0 * kMxSliceBlocks + wave * T::kScaleShare
+                                   : ((int64_t)units_a * slices * kUnitRows + n0) * kMxSliceBlocks +
                                          (wave * T::kScaleShare - T::kScaleA));
     const int lane_c = lane_here();
 #pragma unroll
@@ -263,25 +202,15 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
     if (cur_tile + (int)gridDim.x < total_tiles) cur_tile += gridDim.x;
     begin_cursor();
   };
-  // 16 (4) bytes per lane, one after the other from `to` + OFF
-  auto dma16 = [&](const unsigned char *base, uint32_t offset, uint32_t to, auto off_tag) {
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 ::"s"(to), "v"(offset), "s"(base), "n"(decltype(off_tag)::value) : "memory", "scc");
-  };
-  auto dma4 = [&](const unsigned char *base, uint32_t offset, uint32_t to, auto off_tag) {
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-                 ::"s"(to), "v"(offset), "s"(base), "n"(decltype(off_tag)::value) : "memory", "scc");
-  };
   // LDS addresses of this wave's first region of each half of A, of B and of its scales, in slot 0
   constexpr int kRun = kHalf * 2;   // regions of a half that follow one another
   static_assert(kRun % T::kRegA == 0, "a wave's regions of a half are adjacent");
-  const uint32_t to_a = lds + (uint32_t)(region_row_a(0, 0) * kSliceBytes);
+  const uint32_t to_a = lds + (uint32_t)(region_row_a(0, 0) * kMxSliceBytes);
   const uint32_t to_b = lds + (uint32_t)(T::kOffB + wave * T::kRegB * 1024);
   const uint32_t to_s = lds + (uint32_t)(T::kOffScale + wave * T::kScaleShare);
   auto load_a = [&](auto half_tag, auto q_tag) {
     constexpr int h = decltype(half_tag)::value, q = decltype(q_tag)::value;
-    dma16(at_a, off_a[h * T::kRegA + q], to_a + (uint32_t)(cur_slot * T::kSlotA),
-          std::integral_constant<int, h * kHalf * 16 * kSliceBytes + q * 1024>{});
+    to_lds16<h * kHalf * 16 * kMxSliceBytes + q * 1024>(at_a, off_a[h * T::kRegA + q], to_a + (uint32_t)(cur_slot * T::kSlotA));
   };
   // loads 0 .. kLoadsEarly - 1 of a slice: the lower half of A, B, the scales
   auto load_early = [&](auto x_tag) {
@@ -290,13 +219,12 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
       load_a(std::integral_constant<int, 0>{}, x_tag);
     } else if constexpr (X < T::kRegA + T::kRegB) {
       constexpr int q = X - T::kRegA;
-      dma16(at_b, off_b[q], to_b + (uint32_t)(cur_slot * T::kSlotB), std::integral_constant<int, q * 1024>{});
+      to_lds16<q * 1024>(at_b, off_b[q], to_b + (uint32_t)(cur_slot * T::kSlotB));
     } else if constexpr (T::kScaleLoads == 1) {
-      dma16(at_s, (uint32_t)(lane * 16), to_s + (uint32_t)(cur_slot * T::kScale), std::integral_constant<int, 0>{});
+      to_lds16<0>(at_s, (uint32_t)(lane * 16), to_s + (uint32_t)(cur_slot * T::kScale));
     } else {
       constexpr int part = X - T::kRegA - T::kRegB;
-      dma4(at_s, (uint32_t)(lane * 4 + part * 256), to_s + (uint32_t)(cur_slot * T::kScale),
-           std::integral_constant<int, part * 256>{});
+      to_lds4<part * 256>(at_s, (uint32_t)(lane * 4 + part * 256), to_s + (uint32_t)(cur_slot * T::kScale));
     }
   };
 
@@ -316,11 +244,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
   // the reads of a phase, in the order the next phase uses them
   auto read_a = [&](auto half_tag, uint32_t addr, u32x4(&dst)[kHalf], auto i_tag) {
     constexpr int h = decltype(half_tag)::value, i = decltype(i_tag)::value;
-    read16<(h * kHalf + i) * 16 * kSliceBytes>(addr, dst[i]);
+    read16<(h * kHalf + i) * 16 * kMxSliceBytes>(addr, dst[i]);
   };
   auto read_b = [&](uint32_t addr, u32x4(&dst)[TN], auto j_tag) {
     constexpr int j = decltype(j_tag)::value;
-    read16<j * 16 * kSliceBytes>(addr, dst[j]);
+    read16<j * 16 * kMxSliceBytes>(addr, dst[j]);
   };
   constexpr int kScaleReads = TM / 4 + TN / 4, kNextReads = kHalf + TN + kScaleReads;
   auto read_next = [&](uint32_t aa, uint32_t ba, uint32_t ssa, uint32_t ssb, auto r_tag) {
@@ -361,53 +289,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
   using C0 = std::integral_constant<int, 0>;
   using C1 = std::integral_constant<int, 1>;
 
-  constexpr int kSize = KIND == kElemF32 ? 4 : 2;
-  // The bias of a lane's columns (four adjacent ones of n tile j), as stored; -0 where there is none (the
-  // identity of the add).  It comes through the scalar cache: a vector load would have to wait for every
-  // line that was requested before it.
-  auto bias_of = [&](int n0, auto j_tag, uint32_t(&w)[kSize]) {
-    constexpr int j = decltype(j_tag)::value, kWords = 16 * kSize / 4;
-    const int ge = lane_here() >> 4;
-#pragma unroll
-    for (int e = 0; e < kSize; ++e) w[e] = kSize == 4 ? 0x80000000u : 0x80008000u;
-    if (!p.bias) return;
-    if (n0 + TN * 16 <= p.n && (reinterpret_cast<uintptr_t>(p.bias) & 3u) == 0) {
-      typedef const __attribute__((address_space(4))) uint32_t *ScalarWords;
-      const ScalarWords q = (ScalarWords)(reinterpret_cast<uintptr_t>(p.bias) + (uintptr_t)(n0 + j * 16) * kSize);
-#pragma unroll
-      for (int e = 0; e < kSize; ++e) {
-        const uint32_t low = (ge & 1) ? q[kWords / 4 + e] : q[e];
-        const uint32_t high = (ge & 1) ? q[3 * kWords / 4 + e] : q[kWords / 2 + e];
-        w[e] = (ge & 2) ? high : low;
-      }
-    } else {
-      const int n = n0 + j * 16 + 4 * ge;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.n) {
-          if constexpr (kSize == 4) {
-            w[e] = static_cast<const uint32_t *>(p.bias)[n + e];
-          } else {
-            const uint32_t one = static_cast<const uint16_t *>(p.bias)[n + e];
-            w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | one << 16 : (w[e / 2] & 0xffff0000u) | one;
-          }
-        }
-    }
-  };
-
   for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
     int tm, tn;
     map_tile(tile, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * T::kBM + wm * TM * 16, n0 = tn * T::kBN + wn * TN * 16;   // the wave's part of the tile
-    static_for<0, TN>([&](auto j_tag) {   // the sums start from the bias
-      constexpr int j = decltype(j_tag)::value;
-      uint32_t w[kSize];
-      float b[4];
-      bias_of(n0, j_tag, w);
-      Elem<KIND>::unpack(w, b);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) acc[i][j] = f32x4{b[0], b[1], b[2], b[3]};
-    });
+    start_from_bias<KIND>(p, n0, acc);
     // One slice, in which no branch may stand: behind one the compiler would gather the matrix instructions.
     auto slice = [&]() {
       const uint32_t here_a = lds + (uint32_t)(slot * T::kSlotA) + rd_a0, here_b = lds + (uint32_t)(slot * T::kSlotB) + rd_b0;
@@ -509,97 +395,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
       if (cur_slice == slices) next_tile();
     }
 
-    // ---- the tile's output: slope, rounding, stores ----
-    // A lane holds four adjacent columns (4 ge ..) of row lie of every 16 x 16 tile: 16 bytes in 32 bits.
-    // In 16 bits two n tiles first exchange halves between lanes 16 apart, after which a lane has eight
-    // adjacent columns of one of them.  Either way four lanes hold 64 adjacent bytes of a row, and two
-    // such sets are 128: they exchange rows 8 to 15 of the first for rows 0 to 7 of the second, so that a
-    // store writes eight whole lines.  (With 64 bytes of sixteen rows per store the kernel took 15 % longer.)
-    //
-    // Tiles that lie inside the output as a whole (kInside) store without any test.
-    const int lane_e = lane_here(), lie = lane_e & 15, ge = lane_e >> 4;
-    typedef typename Elem<KIND>::type E;
-    auto outputs = [&](auto slope_tag, auto inside_tag) {
-      constexpr bool kSlope = decltype(slope_tag)::value, kInside = decltype(inside_tag)::value;
-      E *row = static_cast<E *>(p.out) + (int64_t)m0 * p.n + n0;   // wave-uniform
-      constexpr int kSide = 64 / kSize;                            // columns of 64 bytes
-      const int lane_col = (lie >> 3) * kSide + (kSize == 4 ? 4 * ge : (ge & 1) * 16 + (ge >> 1) * 8);
-      const uint32_t lane_at = (uint32_t)((lie & 7) * p.n + lane_col);
-      auto packed = [&](const f32x4 &c, uint32_t(&w)[kSize]) {
-        float v[4] = {c[0], c[1], c[2], c[3]};
-        if constexpr (kSlope) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaxf(v[e], v[e] * p.alpha);
-        }
-        Elem<KIND>::pack(v, w);
-      };
-      // 16 bytes at row m0 + r + lie % 8, column n0 + at + the lane's; `row` points to row m0 + r
-      auto store = [&](int r, int at, u32x4 w) {
-        E *const o = row + at + lane_at;
-        if constexpr (kInside) {
-          __builtin_nontemporal_store(w, reinterpret_cast<u32x4_u *>(o));
-        } else {
-          const int n = n0 + at + lane_col;
-          if (m0 + r + (lie & 7) >= p.m || n >= p.n) return;
-          if (n + 16 / kSize <= p.n) {
-            __builtin_nontemporal_store(w, reinterpret_cast<u32x4_u *>(o));
-          } else {
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 16 / kSize - 1; ++e)
-              if (n + e < p.n) {
-                if constexpr (kSize == 4) o[e] = __uint_as_float(v[e]);
-                else o[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
-              }
-          }
-        }
-      };
-      // `sets` of two times 64 bytes of a row: X and Y
-      auto both = [&](int r, int at, u32x4 x, u32x4 y) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t first = exchange_high(x[e], y[e]), second = exchange_low(x[e], y[e]);
-          x[e] = first;
-          y[e] = second;
-        }
-        store(r, at, x);
-        row += (int64_t)8 * p.n;
-        store(r + 8, at, y);
-        row -= (int64_t)8 * p.n;
-      };
-      static_for<0, TM>([&](auto i_tag) {
-        constexpr int i = decltype(i_tag)::value;
-        if constexpr (kSize == 4) {
-          static_for<0, TN / 2>([&](auto j_tag) {
-            constexpr int j = 2 * decltype(j_tag)::value;
-            uint32_t w0[4], w1[4];
-            packed(acc[i][j], w0);
-            packed(acc[i][j + 1], w1);
-            both(i * 16, j * 16, u32x4{w0[0], w0[1], w0[2], w0[3]}, u32x4{w1[0], w1[1], w1[2], w1[3]});
-          });
-        } else {
-          static_for<0, TN / 4>([&](auto j_tag) {
-            constexpr int j = 4 * decltype(j_tag)::value;
-            u32x4 set[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t w0[2], w1[2];
-              packed(acc[i][j + 2 * h], w0);
-              packed(acc[i][j + 2 * h + 1], w1);
-              // rows of 16 lanes: the odd ones of the first change places with the even ones of the second
-              const u32x2 x = swap_odd_even(w0[0], w1[0]), y = swap_odd_even(w0[1], w1[1]);
-              set[h] = u32x4{x.x, y.x, x.y, y.y};
-            }
-            both(i * 16, j * 16, set[0], set[1]);
-          });
-        }
-        row += (int64_t)16 * p.n;
-      });
-    };
-    const bool inside = m0 + TM * 16 <= p.m && n0 + TN * 16 <= p.n;   // of the wave's rows and columns
-    if (!inside) outputs(std::true_type{}, std::false_type{});
-    else if (p.alpha != 1.f) outputs(std::true_type{}, std::true_type{});
-    else outputs(std::false_type{}, std::true_type{});
+    store_outputs<KIND>(p, m0, n0, acc);
   }
   wait_vmcnt<0>();   // the cursor's last requests still write this workgroup's LDS
 }
@@ -639,7 +435,7 @@ LaunchStatus tiles(const MxOperands &p, void *workspace, uint32_t block_dim, hip
 
 bool mxfp4_dma_supported(const MxOperands &p) {
   // the offset of a lane's line from its tile's first row has 32 bits
-  return p.m > 64 && p.kb >= kSliceBlocks && (int64_t)p.kb * kMxBlockBytes * 256 < (int64_t)1 << 32;
+  return p.m > 64 && p.kb >= kMxSliceBlocks && p.n <= kMxMaxColumns && (int64_t)p.kb * kMxBlockBytes * 256 < (int64_t)1 << 32;
 }
 
 size_t mxfp4_dma_workspace(int64_t m, int64_t kb, int64_t n) {

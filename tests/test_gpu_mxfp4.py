@@ -177,8 +177,41 @@ def test_matmul_on_few_workgroups(H, m, n, k):
     ("bf16", 4096, 4352, 608, 7), ("bf16", 4100, 4090, 256, 0), ("f16", 4300, 4100, 4384, 100), ("bf16", 4352, 4096, 512, 0), ("f32", 4129, 4353, 1312, 200)])
 def test_matmul_on_tiles(H, kind, m, n, k, blocks):
     check_matmul(H, m, n, k, kind, block_dim=blocks)
-    # tiles take whole lines of 256 numbers: shallower products stay on the kernel of few rows
-    assert H.last_launch()["kernel"] == ("mxfp4_matmul_tiles" if k > 224 else "mxfp4_matmul_rows")
+    # the tiled kernels take whole lines of 256 numbers: shallower products stay on the kernel of few rows, and
+    # few tiles go to the kernel with a workgroup per tile
+    few = -(-m // 128) * -(-n // 128) <= 256
+    assert H.last_launch()["kernel"] == ("mxfp4_matmul_rows" if k <= 224 else
+                                         "mxfp4_matmul_ring" if few else "mxfp4_matmul_tiles")
+
+
+@pytest.mark.parametrize("kind,m,n,k,blocks", [
+    # one to many slices of 256, the last one whole or of half the blocks; few and many tiles
+    ("bf16", 65, 64, 256, 0), ("f32", 70, 130, 384, 0), ("f16", 128, 200, 512, 0), ("bf16", 129, 257, 640, 0),
+    ("bf16", 66, 72, 768, 1), ("f32", 200, 100, 1024, 0), ("f16", 257, 520, 1152, 0), ("bf16", 300, 1030, 2176, 3),
+    ("f32", 1000, 2050, 640, 0), ("bf16", 1025, 1796, 1408, 0), ("f16", 2000, 1500, 256, 0), ("bf16", 2048, 2048, 384, 100),
+    ("bf16", 130, 8200, 1024, 0),
+    # scale rows of whole 16-byte pieces, of whole words and of neither; more slices than a tile's scales are held for
+    ("f32", 80, 96, 8192 + 512, 0), ("bf16", 80, 96, 8192 + 384, 0), ("f16", 80, 96, 8192 + 416, 0),
+    ("f32", 257, 130, 16384 + 32, 0), ("f32", 70, 65, 1376, 0), ("bf16", 150, 300, 8192 + 256, 2), ("f32", 66, 70, 255, 0),
+    ("f16", 300, 2048, 992, 0), ("bf16", 500, 4100, 736, 0),
+    # tiles of 32 and 64 rows, below and above a full chip
+    ("bf16", 17, 16, 256, 0), ("f32", 31, 33, 384, 0), ("f16", 32, 8200, 512, 0), ("bf16", 33, 40, 1376, 0),
+    ("f32", 48, 8200, 768, 0), ("bf16", 64, 16400, 1056, 0), ("f16", 64, 32, 8192 + 640, 2), ("bf16", 18, 130, 8192 + 416, 1),
+    ("f32", 40, 24600, 640, 0), ("bf16", 96, 2048, 2048, 0), ("bf16", 64, 8192, 512, 0)])
+def test_matmul_with_a_workgroup_per_tile(H, kind, m, n, k, blocks):
+    check_matmul(H, m, n, k, kind, block_dim=blocks)
+    assert H.last_launch()["kernel"] == "mxfp4_matmul_ring"
+    check_matmul(H, m, n, k, kind, bias=False, alpha=1.0, seed=1)
+
+
+@pytest.mark.parametrize("kind,m,n,k", [("bf16", 4200, 1100, 288), ("f32", 2100, 2100, 512), ("f16", 70, 33000, 256)])
+def test_matmul_without_a_workspace(H, monkeypatch, kind, m, n, k):
+    a = check_matmul(H, m, n, k, kind)
+    monkeypatch.setattr(H, "_workspace", lambda *query: None)
+    b = check_matmul(H, m, n, k, kind)
+    assert H.last_launch()["kernel"] == "mxfp4_matmul_ring"
+    # both add the blocks of a row in one order, onto the bias
+    assert torch.equal(a, b)
 
 
 def test_matmul_without_depth_is_the_bias(H):
