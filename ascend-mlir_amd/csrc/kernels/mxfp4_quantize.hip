@@ -116,9 +116,10 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows(const void *__re
           if (at[u] + 8 <= k) {
             uint32_t o[kWords];
             Elem<KIND>::pack(back, o);
-            *reinterpret_cast<u32x4_u *>(p) = u32x4{o[0], o[1], o[2], o[3]};
+            __builtin_nontemporal_store(u32x4{o[0], o[1], o[2], o[3]}, reinterpret_cast<u32x4_u *>(p));
             if constexpr (kWords == 8)
-              *reinterpret_cast<u32x4_u *>(p + 4) = u32x4{o[kWords - 4], o[kWords - 3], o[kWords - 2], o[kWords - 1]};
+              __builtin_nontemporal_store(u32x4{o[kWords - 4], o[kWords - 3], o[kWords - 2], o[kWords - 1]},
+                                          reinterpret_cast<u32x4_u *>(p + 4));
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -134,7 +135,10 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows(const void *__re
 // A workgroup takes 256 rows of 64 lanes' columns; a wavefront takes 32 of the rows, one block of
 // every column, and a lane holds the block of its own one or two columns (4 bytes of a row) in
 // registers: 32 loads in flight, each a contiguous piece of a row, and no exchange between lanes.
-// The eight blocks of a column meet in LDS and leave as whole 128-byte lines of its code row.
+// The eight blocks of a column meet in LDS and leave as whole 128-byte lines of its code row.  Rows that
+// are no whole number of lines share lines between neighbouring tiles, which therefore belong to one XCD,
+// whose L2 puts them together: float32 [8192, 4099] with values 54 us (5.3 TB/s) against 72 with
+// neighbours on different XCDs (and 71 with stores that bypass the L2).
 constexpr int kColWaves = 8;
 template <int KIND, bool VALUES>
 __global__ __launch_bounds__(kColWaves * 64) void mxfp4_quantize_cols(const void *__restrict__ x, int64_t ld,
@@ -148,7 +152,11 @@ __global__ __launch_bounds__(kColWaves * 64) void mxfp4_quantize_cols(const void
   __shared__ __align__(16) u32x4 code_tile[kCols * kColWaves];
   __shared__ __align__(8) uint8_t scale_tile[kCols * kColWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  // workgroup i runs on XCD i % 8, and an XCD takes tiles that follow one another
+  const int64_t per_xcd = (tiles + kNumXCD - 1) / kNumXCD;
+  for (int64_t q = blockIdx.x; q < per_xcd * kNumXCD; q += gridDim.x) {
+    const int64_t tile = q % kNumXCD * per_xcd + q / kNumXCD;
+    if (tile >= tiles) continue;
     const int64_t c0 = (tile % tiles_r) * kCols, b0 = (tile / tiles_r) * kColWaves;
     const int64_t c = c0 + lane * VC, k0 = (b0 + wave) * kMxBlock;
     uint32_t w[kMxBlock];
@@ -271,7 +279,8 @@ LaunchStatus quantize_cols(const void *x, int64_t ld, void *codes, void *scales,
   constexpr int kCols = 64 * (Elem<KIND>::kPer16 / 4);
   const int64_t kb = (k + kMxBlock - 1) / kMxBlock;
   const int64_t tiles_r = (r + kCols - 1) / kCols, tiles = tiles_r * ((kb + kColWaves - 1) / kColWaves);
-  int64_t grid = tiles < (int64_t)1 << 20 ? tiles : (int64_t)1 << 20;
+  const int64_t places = (tiles + kNumXCD - 1) / kNumXCD * kNumXCD;
+  int64_t grid = places < (int64_t)1 << 20 ? places : (int64_t)1 << 20;
   if (block_dim) grid = block_dim;
   AFIR_LAUNCH("mxfp4_quantize_cols", (mxfp4_quantize_cols<KIND, VALUES>), dim3((unsigned)grid), dim3(kColWaves * 64), 0,
               stream, x, ld, static_cast<unsigned char *>(codes), static_cast<uint8_t *>(scales), values, k, r, kb,
