@@ -19,6 +19,8 @@ namespace afir {
 
 namespace {
 
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+
 // What a lane holds of a row: ITEMS 16-byte pieces, lanes adjacent.
 template <int KIND, int ITEMS>
 struct Piece {
@@ -28,13 +30,13 @@ struct Piece {
 // Row pieces of a lane; numbers past the row's end are zeros and add nothing to any sum.  (A
 // 16-byte access needs the alignment of an element only, see mxfp4.h.)
 template <int KIND, int LANES, int ITEMS>
-__device__ __forceinline__ void load_row(const void *base, int64_t offset, int lane, int64_t n, Piece<KIND, ITEMS> &p) {
+__device__ __forceinline__ void load_row(const void *base, int64_t offset, int lane, uint32_t n, Piece<KIND, ITEMS> &p) {
   constexpr int V = Elem<KIND>::kPer16;
   typedef typename Elem<KIND>::type T;
   const T *row = static_cast<const T *>(base) + offset;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int64_t e = (int64_t)(lane + i * LANES) * V;
+    const uint32_t e = (uint32_t)(lane + i * LANES) * V;   // (32-bit: the row's start stays a scalar)
     p.w[i][0] = p.w[i][1] = p.w[i][2] = p.w[i][3] = 0;
     if (e + V <= n) {
       const u32x4 v = *reinterpret_cast<const u32x4_u *>(row + e);
@@ -50,7 +52,7 @@ __device__ __forceinline__ void load_row(const void *base, int64_t offset, int l
   }
 }
 template <int KIND, int LANES>
-__device__ __forceinline__ void store_item(void *base, int64_t offset, int64_t e, int64_t n,
+__device__ __forceinline__ void store_item(void *base, int64_t offset, uint32_t e, uint32_t n,
                                            const float (&v)[Elem<KIND>::kPer16]) {
   constexpr int V = Elem<KIND>::kPer16;
   typedef typename Elem<KIND>::type T;
@@ -96,6 +98,11 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], float *lds, int &tur
   }
 }
 
+// (at most 2^31 rows, and the launch holds rows_per_gate to them: a 64-bit division is some 100 instructions)
+__device__ __forceinline__ int64_t gate_row(int64_t row, int64_t rows_per_gate) {
+  return (uint32_t)row / (uint32_t)rows_per_gate;
+}
+
 __device__ __forceinline__ float rstd_of(float sum_of_squares, float inv_n, float eps) {
   return 1.0f / sqrtf(sum_of_squares * inv_n + eps);
 }
@@ -108,7 +115,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateA
   constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64, kRowsHere = threads_of(WAVES) / kLanes;
   __shared__ __align__(16) float lds[2 * WAVES * 4];
   const int lane = threadIdx.x % kLanes, wave = lane >> 6;
-  const int64_t n = p.n;
+  const uint32_t n = (uint32_t)p.n;
   Piece<KIND, ITEMS> post, pre;
   if (p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
   if (p.h) load_row<KIND, kLanes, ITEMS>(p.pre_weight, 0, lane, n, pre);
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateA
     load_row<KIND, kLanes, ITEMS>(p.x, r * p.ld_x, lane, n, x);
     if (p.f) {
       load_row<KIND, kLanes, ITEMS>(p.f, r * p.ld_f, lane, n, f);
-      if (p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      if (p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(r, p.rows_per_gate) * p.ld_gate, lane, n, gate);
     }
   };
   if (row < p.m) fetch(row);
@@ -158,7 +165,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateA
     if (p.y)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i)
-        store_item<KIND, kLanes>(p.y, row * p.ld_y, (int64_t)(lane + i * kLanes) * V, n, y[i]);
+        store_item<KIND, kLanes>(p.y, row * p.ld_y, (uint32_t)(lane + i * kLanes) * V, n, y[i]);
     if (p.h) {
       float sum[1] = {0.f};
 #pragma unroll
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void norm_gate_forward(NormGateA
         Elem<KIND>::unpack(pre.w[i], vw);
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = y[i][j] * ry * vw[j];
-        store_item<KIND, kLanes>(p.h, row * p.ld_h, (int64_t)(lane + i * kLanes) * V, n, o);
+        store_item<KIND, kLanes>(p.h, row * p.ld_h, (uint32_t)(lane + i * kLanes) * V, n, o);
       }
     }
   }
@@ -221,27 +228,34 @@ LaunchStatus forward(const NormGateArgs &p, uint32_t block_dim, hipStream_t stre
 // the gate is one row throughout (kOneGate: the partial sum is that of t fn, which serves dgate
 // and, weighted with the gate, dpost_weight), or dgate's rows are finished within the workgroup.
 struct Stretches {       // stretch i: rows from (i / per_span) * span + (i % per_span) * rows
-  int64_t span;          // rows of one gate row, or of several whole ones
-  int64_t per_span, rows, count;
+  uint32_t span;         // rows of one gate row, or of several whole ones
+  uint32_t per_span, rows, count;
   bool one_gate;
 };
 
 inline Stretches plan_stretches(int64_t m, int64_t rows_per_gate, bool gate, int64_t workgroups) {
+  const int64_t rows = (m + workgroups - 1) / workgroups, per_gate = gate && rows_per_gate < m ? rows_per_gate : m;
+  const bool whole = gate && per_gate <= rows;   // gate rows, as many as fit
+  const int64_t span = whole ? rows / per_gate * per_gate : per_gate, per_span = whole ? 1 : (per_gate + rows - 1) / rows;
   Stretches s;
-  int64_t rows = (m + workgroups - 1) / workgroups;
-  const int64_t per_gate = gate && rows_per_gate < m ? rows_per_gate : m;
-  if (gate && per_gate <= rows) {
-    s.one_gate = per_gate == m;
-    s.rows = s.span = rows / per_gate * per_gate;
-    s.per_span = 1;
-  } else {
-    s.one_gate = true;
-    s.span = per_gate;
-    s.per_span = (per_gate + rows - 1) / rows;
-    s.rows = (per_gate + s.per_span - 1) / s.per_span;
-  }
-  s.count = (m + s.span - 1) / s.span * s.per_span;
+  s.one_gate = !whole || per_gate == m;
+  s.span = (uint32_t)span;
+  s.per_span = (uint32_t)per_span;
+  s.rows = (uint32_t)((span + per_span - 1) / per_span);
+  s.count = (uint32_t)((m + span - 1) / span * per_span);
   return s;
+}
+
+template <int V>
+__device__ __forceinline__ void store_sums(float *row, uint32_t e, uint32_t n, const float (&v)[V]) {
+  if (e + V <= n) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) *reinterpret_cast<f32x4_u *>(row + e + j) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < V - 1; ++j)
+      if (e + j < n) row[e + j] = v[j];
+  }
 }
 
 template <int KIND, int WAVES, int ITEMS, bool kOneGate>
@@ -250,13 +264,13 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
   constexpr bool kAhead = ITEMS == 1;
   __shared__ __align__(16) float lds[2 * WAVES * 4];
   const int lane = threadIdx.x, wave = lane >> 6;
-  const int64_t n = p.n;
+  const uint32_t n = (uint32_t)p.n;
   Piece<KIND, ITEMS> post, pre;
-  if (p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
+  if (!kOneGate && p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
   if (p.dh) load_row<KIND, kLanes, ITEMS>(p.pre_weight, 0, lane, n, pre);
   int turn = 0;
-  for (int64_t stretch = blockIdx.x; stretch < s.count; stretch += gridDim.x) {
-    const int64_t first = stretch / s.per_span * s.span, r0 = first + stretch % s.per_span * s.rows;
+  for (uint32_t stretch = blockIdx.x; stretch < s.count; stretch += gridDim.x) {
+    const int64_t first = (int64_t)(stretch / s.per_span) * s.span, r0 = first + (int64_t)(stretch % s.per_span) * s.rows;
     int64_t r1 = r0 + s.rows < first + s.span ? r0 + s.rows : first + s.span;
     r1 = r1 < p.m ? r1 : p.m;
     float acc_post[ITEMS][V], acc_pre[ITEMS][V], acc_gate[kOneGate ? 1 : ITEMS][V];
@@ -276,26 +290,54 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
       }
       if (p.f) {
         load_row<KIND, kLanes, ITEMS>(p.f, r * p.ld_f, lane, n, f);
-        if (!kOneGate && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+        if (!kOneGate && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(r, p.rows_per_gate) * p.ld_gate, lane, n, gate);
       }
     };
     if (r0 < r1) {
-      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, (r0 / p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      if (kOneGate && p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
+      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(r0, p.rows_per_gate) * p.ld_gate, lane, n, gate);
       fetch(r0);
     }
+    // gate post_weight: held through the stretch where it is one row and there are registers for it
+    constexpr bool kHeld = kOneGate && ITEMS == 1;
+    float held[V];
+    auto weights = [&](int i, const Piece<KIND, ITEMS> &gate_now, float (&w)[V]) {
+      float vg[V];
+      Elem<KIND>::unpack(post.w[i], w);
+      if (!p.gate) return;
+      Elem<KIND>::unpack(gate_now.w[i], vg);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] *= vg[j];
+    };
+    if (kHeld && p.f && r0 < r1) weights(0, gate, held);
+    auto weight_row = [&](int i, const Piece<KIND, ITEMS> &gate_now, float (&w)[V]) {
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = held[j];
+      } else {
+        weights(i, gate_now, w);
+      }
+    };
+    auto unpack_a = [&](int i, float (&v)[V]) {   // a = dh pre_weight
+      float vw[V];
+      Elem<KIND>::unpack(dh.w[i], v);
+      Elem<KIND>::unpack(pre.w[i], vw);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= vw[j];
+    };
     for (int64_t row = r0; row < r1; ++row) {
-      float sums[3] = {0.f, 0.f, 0.f};   // y^2, dh pre y, f^2
+      float sums[3] = {0.f, 0.f, 0.f};   // y^2, a y, f^2
+      float a[V], t[ITEMS][V];   // (a stays where there are registers, or is formed anew)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         if (p.dh) {
-          float vy[V], vd[V], vw[V];
+          float vy[V];
           Elem<KIND>::unpack(y.w[i], vy);
-          Elem<KIND>::unpack(dh.w[i], vd);
-          Elem<KIND>::unpack(pre.w[i], vw);
+          unpack_a(i, a);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             sums[0] += vy[j] * vy[j];
-            sums[1] += vd[j] * vw[j] * vy[j];
+            sums[1] += a[j] * vy[j];
           }
         }
         if (p.f) {
@@ -308,8 +350,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
       row_sums<WAVES>(sums, lds, turn, wave);
       const float ry = rstd_of(sums[0], p.inv_n, p.eps), rf = rstd_of(sums[2], p.inv_n, p.eps);
       const float my = ry * sums[1] * p.inv_n;   // mean(a yn)
-      float t[ITEMS][V];
-      float dot[1] = {0.f};
+      float dot[1] = {0.f};                      // b f
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         if (p.dy) Elem<KIND>::unpack(dy.w[i], t[i]);
@@ -317,32 +358,31 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
 #pragma unroll
           for (int j = 0; j < V; ++j) t[i][j] = 0.f;
         if (p.dh) {
-          float vy[V], vd[V], vw[V];
+          float vy[V], vd[V];
           Elem<KIND>::unpack(y.w[i], vy);
           Elem<KIND>::unpack(dh.w[i], vd);
-          Elem<KIND>::unpack(pre.w[i], vw);
+          if (ITEMS > 1 || !kOneGate) unpack_a(i, a);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const float yn = vy[j] * ry;
-            t[i][j] += ry * (vd[j] * vw[j] - yn * my);
+            t[i][j] += ry * (a[j] - yn * my);
             acc_pre[i][j] += vd[j] * yn;
           }
         }
         if (p.f) {
           float vf[V], vg[V], vw[V];
           Elem<KIND>::unpack(f.w[i], vf);
-          Elem<KIND>::unpack(post.w[i], vw);
-          if (p.gate) Elem<KIND>::unpack(gate.w[i], vg);
+          weight_row(i, gate, vw);
+          if (!kOneGate && p.gate) Elem<KIND>::unpack(gate.w[i], vg);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float gt = p.gate ? vg[j] * t[i][j] : t[i][j];
-            const float fn = vf[j] * rf;
-            dot[0] += gt * vw[j] * fn;
+            const float tf = t[i][j] * (vf[j] * rf);
+            dot[0] += t[i][j] * vw[j] * vf[j];
             if constexpr (kOneGate) {
-              acc_post[i][j] += t[i][j] * fn;
+              acc_post[i][j] += tf;
             } else {
-              acc_post[i][j] += gt * fn;
-              acc_gate[i][j] += t[i][j] * fn;
+              acc_post[i][j] += p.gate ? vg[j] * tf : tf;
+              acc_gate[i][j] += tf;
             }
           }
         }
@@ -356,26 +396,22 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = p.residual_scale * t[i][j];
-        store_item<KIND, kLanes>(p.dx, row * p.ld_dx, (int64_t)(lane + i * kLanes) * V, n, o);
+        store_item<KIND, kLanes>(p.dx, row * p.ld_dx, (uint32_t)(lane + i * kLanes) * V, n, o);
       }
       if (p.f) {
         row_sums<WAVES>(dot, lds, turn, wave);
-        const float mf = dot[0] * p.inv_n;   // mean(b fn)
+        const float mf = rf * dot[0] * p.inv_n;   // mean(b fn)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-          float o[V], vf[V], vg[V], vw[V];
+          float o[V], vf[V], vw[V];
           Elem<KIND>::unpack(f_here.w[i], vf);
-          Elem<KIND>::unpack(post.w[i], vw);
-          if (p.gate) Elem<KIND>::unpack(gate_here.w[i], vg);
+          weight_row(i, gate_here, vw);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float b = (p.gate ? vg[j] * t[i][j] : t[i][j]) * vw[j];
-            o[j] = rf * (b - vf[j] * rf * mf);
-          }
-          store_item<KIND, kLanes>(p.df, row * p.ld_df, (int64_t)(lane + i * kLanes) * V, n, o);
+          for (int j = 0; j < V; ++j) o[j] = rf * (t[i][j] * vw[j] - vf[j] * rf * mf);
+          store_item<KIND, kLanes>(p.df, row * p.ld_df, (uint32_t)(lane + i * kLanes) * V, n, o);
         }
         if constexpr (!kOneGate) {
-          if ((row + 1) % p.rows_per_gate == 0 || row + 1 == p.m) {
+          if ((uint32_t)(row + 1) % (uint32_t)p.rows_per_gate == 0 || row + 1 == p.m) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
               float o[V], vw[V];
@@ -385,70 +421,80 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
                 o[j] = acc_gate[i][j] * vw[j];
                 acc_gate[i][j] = 0.f;
               }
-              store_item<KIND, kLanes>(p.dgate, row / p.rows_per_gate * n, (int64_t)(lane + i * kLanes) * V, n, o);
+              store_item<KIND, kLanes>(p.dgate, gate_row(row, p.rows_per_gate) * p.n, (uint32_t)(lane + i * kLanes) * V, n, o);
             }
           }
         }
       }
       if (!kAhead && row + 1 < r1) fetch(row + 1);
     }
-    float *const part_post = p.partial + stretch * n, *const part_pre = p.partial + (s.count + stretch) * n;
+    float *const part_post = p.partial + (int64_t)stretch * p.n, *const part_pre = p.partial + ((int64_t)s.count + stretch) * p.n;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int64_t e = (int64_t)(lane + i * kLanes) * V + j;
-        if (e < n) {
-          if (p.f) part_post[e] = acc_post[i][j];
-          if (p.dh) part_pre[e] = acc_pre[i][j];
-        }
-      }
+    for (int i = 0; i < ITEMS; ++i) {
+      const uint32_t e = (uint32_t)(lane + i * kLanes) * V;
+      if (p.f) store_sums(part_post, e, n, acc_post[i]);
+      if (p.dh) store_sums(part_pre, e, n, acc_pre[i]);
+    }
   }
 }
 
 // Adds the partial rows: blockIdx.y 0 gives dpre_weight, 1 dpost_weight, 2 + g gate row g (kOneGate
-// launches with a gate).  64 columns per workgroup, four to a lane; 64 groups of lanes share the rows,
-// and their sums are added in order.
-constexpr int kJoinGroups = 64;
-typedef f32x4 f32x4_u __attribute__((aligned(4)));
+// launches with a gate).  32 columns per workgroup, a line of a partial row, four to a lane; 64 groups of
+// lanes share the rows, eight rows in flight each.  Their sums are added in a fixed order: the groups of a
+// wavefront across its lanes, the wavefronts through LDS.
+constexpr int kJoinColumns = 32, kJoinLanes = kJoinColumns / 4, kJoinGroups = 64, kJoinWaves = kJoinGroups * kJoinLanes / 64;
 template <int KIND>
-__global__ __launch_bounds__(kJoinGroups * 16) void norm_gate_join(NormGateGradArgs p, Stretches s, int64_t column_tiles) {
-  __shared__ f32x4 lds[kJoinGroups][16];
-  const int four = threadIdx.x & 15, group = threadIdx.x >> 4;
+__global__ __launch_bounds__(kJoinWaves * 64) void norm_gate_join(NormGateGradArgs p, Stretches s, int64_t column_tiles) {
+  __shared__ f32x4 lds[kJoinWaves][kJoinLanes];
+  const int four = threadIdx.x % kJoinLanes, group = threadIdx.x / kJoinLanes;
   const int what = blockIdx.y;
   if ((what == 0 && !p.dh) || (what == 1 && !p.f)) return;
-  const float *const part = p.partial + (what == 0 ? s.count * p.n : 0);
-  const int64_t first = what < 2 ? 0 : (what - 2) * s.per_span, last = what < 2 ? s.count : first + s.per_span;
+  const float *const part = p.partial + (what == 0 ? (int64_t)s.count * p.n : 0);
+  const uint32_t first = what < 2 ? 0 : (what - 2) * s.per_span, last = what < 2 ? s.count : first + s.per_span;
   const bool weighted = what == 1 && s.one_gate && p.gate;
   for (int64_t tile = blockIdx.x; tile < column_tiles; tile += gridDim.x) {
-    const int64_t e0 = tile * 64 + four * 4;
+    const int64_t e0 = tile * kJoinColumns + four * 4;
     const int here = p.n - e0 < 4 ? (p.n > e0 ? (int)(p.n - e0) : 0) : 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int64_t r = first + group; r < last; r += kJoinGroups) {
+    auto add = [&](uint32_t r, auto weighted_tag) {
       f32x4 x = {0.f, 0.f, 0.f, 0.f}, w = {1.f, 1.f, 1.f, 1.f};
       if (here == 4) {
-        x = *reinterpret_cast<const f32x4_u *>(part + r * p.n + e0);
+        x = *reinterpret_cast<const f32x4_u *>(part + (int64_t)r * p.n + e0);
       } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-          if (j < here) x[j] = part[r * p.n + e0 + j];
+          if (j < here) x[j] = part[(int64_t)r * p.n + e0 + j];
       }
-      if (weighted) {
+      if constexpr (decltype(weighted_tag)::value) {
+        const int64_t at = (int64_t)(r / s.per_span) * p.ld_gate + e0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (j < here) w[j] = Elem<KIND>::load(p.gate, r / s.per_span * p.ld_gate + e0 + j);
+          if (j < here) w[j] = Elem<KIND>::load(p.gate, at + j);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += x[j] * w[j];
-    }
-    lds[group][four] = v;
-    __syncthreads();
-    const int64_t e = tile * 64 + threadIdx.x;
-    if (threadIdx.x < 64 && e < p.n) {
-      float sum = 0.f;
+    };
+    if (weighted) {
+#pragma unroll 4
+      for (uint32_t r = first + group; r < last; r += kJoinGroups) add(r, std::true_type{});
+    } else {
 #pragma unroll 8
-      for (int w = 0; w < kJoinGroups; ++w) sum += reinterpret_cast<const float *>(lds[w])[threadIdx.x];
+      for (uint32_t r = first + group; r < last; r += kJoinGroups) add(r, std::false_type{});
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // lanes 8, 16 and 32 apart hold the same columns
+      v[j] += __shfl_xor(v[j], 8);
+      v[j] += __shfl_xor(v[j], 16);
+      v[j] += __shfl_xor(v[j], 32);
+    }
+    if ((threadIdx.x & 63) < kJoinLanes) lds[threadIdx.x >> 6][four] = v;
+    __syncthreads();
+    const int64_t e = tile * kJoinColumns + threadIdx.x;
+    if (threadIdx.x < kJoinColumns && e < p.n) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWaves; ++w) sum += reinterpret_cast<const float *>(lds[w])[threadIdx.x];
       if (what == 0) Elem<KIND>::store(p.dpre_weight, e, sum);
       else if (what == 1) Elem<KIND>::store(p.dpost_weight, e, sum);
       else Elem<KIND>::store(p.dgate, (what - 2) * p.n + e, sum * Elem<KIND>::load(p.post_weight, e));
@@ -484,10 +530,10 @@ LaunchStatus backward_launch(const NormGateGradArgs &p, const Stretches &s, uint
                 dim3(WAVES * 64), 0, stream, p, s);
   const LaunchStatus st = after_launch();
   if (st.code) return st;
-  const int64_t column_tiles = (p.n + 63) / 64;
+  const int64_t column_tiles = (p.n + kJoinColumns - 1) / kJoinColumns;
   const int64_t gates = s.one_gate && p.f && p.gate ? (p.m + p.rows_per_gate - 1) / p.rows_per_gate : 0;
   AFIR_LAUNCH("norm_gate_join", (norm_gate_join<KIND>), dim3((unsigned)column_tiles, (unsigned)(2 + gates)),
-              dim3(kJoinGroups * 16), 0, stream, p, s, column_tiles);
+              dim3(kJoinWaves * 64), 0, stream, p, s, column_tiles);
   return after_launch();
 }
 
@@ -530,6 +576,7 @@ LaunchStatus launch_norm_gate_residual(const NormGateArgs &args, int elem_kind, 
   for (const void *q : {p.x, p.f, p.gate, p.post_weight, p.pre_weight, (const void *)p.y, (const void *)p.h})
     if (reinterpret_cast<uintptr_t>(q) % elem) return invalid("norm_gate_residual: tensor off its element's alignment");
   p.inv_n = (float)(1.0 / (double)p.n);
+  if (p.rows_per_gate > p.m) p.rows_per_gate = p.m;
   switch (elem_kind) {
     case kElemF32: return forward<kElemF32>(p, block_dim, stream);
     case kElemF16: return forward<kElemF16>(p, block_dim, stream);
@@ -574,6 +621,7 @@ LaunchStatus launch_norm_gate_residual_backward(const NormGateGradArgs &args, in
       return invalid("norm_gate_residual_backward: tensor off its element's alignment");
   if (reinterpret_cast<uintptr_t>(p.partial) % 4) return invalid("norm_gate_residual_backward: workspace off a 4-byte boundary");
   p.inv_n = (float)(1.0 / (double)p.n);
+  if (p.rows_per_gate > p.m) p.rows_per_gate = p.m;
   switch (elem_kind) {
     case kElemF32: return backward<kElemF32>(p, block_dim, stream);
     case kElemF16: return backward<kElemF16>(p, block_dim, stream);
