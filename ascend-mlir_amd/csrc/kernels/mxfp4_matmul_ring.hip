@@ -89,26 +89,28 @@ mxfp4_matmul_ring(MxOperands p, int slices, ScaleRows how, int tiles_m, int tile
       const int row = of_a ? m0 + r : n0 + r - T::kBM, rows = of_a ? p.m : p.n;
       return (of_a ? p.a_scales : p.b_scales) + (int64_t)(row < rows ? row : rows - 1) * p.kb;
     };
-    // (a row takes 2^row_log bytes of LDS, a power of two of pieces)
+    // A row takes 2^row_log bytes of LDS, a power of two of pieces.  Piece c of row r is at c ^ (r >> (4 - piece_log)):
+    // rows that share banks differ in it.
     const int held = slices < kScaleSlices ? slices : kScaleSlices;
     const int piece_log = 31 - __builtin_clz((unsigned)((held + 1) / 2 * 2 - 1)), row_log = piece_log + 4;
     const int piece_mask = (1 << piece_log) - 1;
+    auto place_of = [&](int r, int c) { return ((r >> (4 - piece_log)) ^ c) & piece_mask; };   // and back
     auto load_scales = [&](int first) {
       const int block0 = first * kMxSliceBlocks;
       const uint32_t to = lds + (uint32_t)T::kOffScale;
       const int per_load = how == kPieces ? 6 - piece_log : 4 - piece_log;   // log2 of the rows of one load
       for (int i = wave; i << per_load < T::kRows; i += T::kWaves) {   // (rows past the last repeat it)
         if (how == kPieces) {
-          const int r = (i << per_load) + (lane >> piece_log), at = block0 + (((lane ^ r) & piece_mask) << 4);
+          const int r = (i << per_load) + (lane >> piece_log), at = block0 + (place_of(r, lane) << 4);
           to_lds16_at(scale_row(r) + (at <= p.kb - 16 ? at : p.kb - 16), to + (uint32_t)(i * 1024));
         } else {
           const int r = (i << per_load) + (lane >> (piece_log + 2));
-          const int at = block0 + ((((lane >> 2) ^ r) & piece_mask) << 4) + (lane & 3) * 4;
+          const int at = block0 + (place_of(r, lane >> 2) << 4) + (lane & 3) * 4;
           to_lds4_at(scale_row(r) + (at <= p.kb - 4 ? at : p.kb - 4), to + (uint32_t)(i * 256));
         }
       }
     };
-    auto piece_of = [&](int r, int c) { return T::kOffScale + (r << row_log) + (((c ^ r) & piece_mask) << 4); };
+    auto piece_of = [&](int r, int c) { return T::kOffScale + (r << row_log) + (place_of(r, c) << 4); };
     // a last slice of four blocks (rows of whole words) has them in its first word: they belong in the second
     auto shift_last = [&](int s) {
       for (int r = t; r < T::kRows; r += T::kWaves * 64) {
@@ -162,7 +164,7 @@ mxfp4_matmul_ring(MxOperands p, int slices, ScaleRows how, int tiles_m, int tile
       uint32_t a, b, sa, sb;
     };
     auto places = [&](int slot, int s) {   // of slice s of those whose scales are in LDS
-      const uint32_t piece = (uint32_t)(((((s >> 1) ^ li) & piece_mask) << 4) | ((s & 1) << 3)), at = lds + (uint32_t)(slot * T::kSlot);
+      const uint32_t piece = (uint32_t)((place_of(li, s >> 1) << 4) | ((s & 1) << 3)), at = lds + (uint32_t)(slot * T::kSlot);
       return Places{at + rd_a, at + rd_b, lds + rd_sa + piece, lds + rd_sb + piece};
     };
     // one of a slice's reads: first the scales, then the first and the second step's codes

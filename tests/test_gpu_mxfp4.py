@@ -197,6 +197,10 @@ def test_matmul_on_tiles(H, kind, m, n, k, blocks):
     # tiles of 32 and 64 rows, below and above a full chip
     ("bf16", 17, 16, 256, 0), ("f32", 31, 33, 384, 0), ("f16", 32, 8200, 512, 0), ("bf16", 33, 40, 1376, 0),
     ("f32", 48, 8200, 768, 0), ("bf16", 64, 16400, 1056, 0), ("f16", 64, 32, 8192 + 640, 2), ("bf16", 18, 130, 8192 + 416, 1),
+    # more slices than the scales held: 1 to 32 of them beyond, rows of scales whole, of words and of bytes
+    ("f32", 40, 70, 8192 + 4096, 0), ("bf16", 65, 64, 8192 + 512, 0), ("f16", 150, 260, 8192 + 4096 + 128, 0),
+    ("bf16", 33, 100, 16384, 0), ("f32", 70, 40, 16384 + 256, 1), ("bf16", 20, 48, 16384 + 4096 + 32, 0),
+    ("f16", 260, 4100, 8192 + 2048 + 384, 0), ("f32", 130, 130, 4096 + 96, 0), ("bf16", 40, 40, 4096 + 128, 0),
     ("f32", 40, 24600, 640, 0), ("bf16", 96, 2048, 2048, 0), ("bf16", 64, 8192, 512, 0)])
 def test_matmul_with_a_workgroup_per_tile(H, kind, m, n, k, blocks):
     check_matmul(H, m, n, k, kind, block_dim=blocks)
