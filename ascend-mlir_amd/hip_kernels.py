@@ -330,9 +330,15 @@ def _rows(t, shape, dtype, index, what):
     return ld
 
 
-def _launch_on(index, symbol, block_dim, stream, tiling, workspace, *tensors):
-    """Launch with device `index` current; tensors may be None.  The stream is the caller's
-    or the current one of that device."""
+def _given_stream(stream, index):
+    """The caller's stream as the current one, for a call's results and scratch as well: memory
+    from another stream's pool may still be in use by work that is under way there."""
+    import torch
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=index))
+
+
+def _launch_on(index, symbol, block_dim, tiling, workspace, *tensors):
+    """Launch on the current stream of device `index`; tensors may be None."""
     import torch
     fn = _entries.get(symbol)
     if fn is None:
@@ -340,19 +346,17 @@ def _launch_on(index, symbol, block_dim, stream, tiling, workspace, *tensors):
     ptrs = [None if t is None else t.data_ptr() for t in tensors]
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            st = torch.cuda.current_stream(index).cuda_stream if stream is None else stream
-            rc = fn(block_dim, st, *ptrs, workspace, tiling)
+            rc = fn(block_dim, torch._C._cuda_getCurrentRawStream(index), *ptrs, workspace, tiling)
     else:
         # (the raw handle: building a Stream object takes as long as the rest of the call)
-        st = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream
-        rc = fn(block_dim, st, *ptrs, workspace, tiling)
+        rc = fn(block_dim, torch._C._cuda_getCurrentRawStream(index), *ptrs, workspace, tiling)
     if rc:
         _check(rc)
 
 
-def _workspace(query, tiling, like, stream):
+def _workspace(query, tiling, like):
     """Scratch of the size that the library asks for, from torch's allocator, which hands it
-    out again only to work that follows on the stream of this call."""
+    out again only to work that follows on the current stream, that of this call."""
     import torch
     fn = _entries.get(query)
     if fn is None:
@@ -360,10 +364,7 @@ def _workspace(query, tiling, like, stream):
     size = fn(tiling)
     if not size:
         return None
-    ws = torch.empty((size,), dtype=torch.uint8, device=like.device)
-    if stream is not None:
-        ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
-    return ws
+    return torch.empty((size,), dtype=torch.uint8, device=like.device)
 
 
 _PACK5, _PACK11, _PACK13 = (struct.Struct(f"<{count}q").pack for count in (5, 11, 13))
@@ -380,6 +381,9 @@ def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_valu
     Blocks that hold an infinity or a NaN read as NaN throughout."""
     import torch
     index = _device_of(x, "x")
+    if stream is not None:
+        with _given_stream(stream, index):
+            return mxfp4_quantize(x, axis, codes, scales, values, return_values, block_dim)
     if x.dim() != 2:
         raise AfirHipError("mxfp4_quantize: x must have two dimensions")
     if axis not in (-1, 0, 1):
@@ -401,7 +405,7 @@ def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_valu
         _dense(values, shape, dtype, index, "values")
     elif return_values:
         values = torch.empty(shape, dtype=dtype, device=x.device)
-    _launch_on(index, "afir_hip_launch_mxfp4_quantize", block_dim, stream,
+    _launch_on(index, "afir_hip_launch_mxfp4_quantize", block_dim,
                _PACK5(shape[0], shape[1], ld, 0 if axis == 0 else 1, kind), None, x, codes, scales, values)
     return (codes, scales) if values is None else (codes, scales, values)
 
@@ -414,6 +418,9 @@ def mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias=None, alpha=0.01, 
     32 (only checked against the codes)."""
     import torch
     index = _device_of(a, "a")
+    if stream is not None:
+        with _given_stream(stream, index):
+            return mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias, alpha, out, out_dtype, k, block_dim)
     try:
         (m, row), (n, _) = a.shape, b.shape
     except (AttributeError, ValueError):
@@ -440,8 +447,8 @@ def mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias=None, alpha=0.01, 
     if bias is not None:
         _dense(bias, (n,), dtype, index, "bias")
     tiling = _PACK5(m, k, n, f32_bits(alpha), kind)
-    ws = _workspace("afir_hip_mxfp4_matmul_workspace_bytes", tiling, a, stream)
-    _launch_on(index, "afir_hip_launch_mxfp4_matmul_add_leakyrelu", block_dim, stream, tiling,
+    ws = _workspace("afir_hip_mxfp4_matmul_workspace_bytes", tiling, a)
+    _launch_on(index, "afir_hip_launch_mxfp4_matmul_add_leakyrelu", block_dim, tiling,
                None if ws is None else ws.data_ptr(), a, a_scales, b, b_scales, bias, out)
     return out
 
@@ -476,6 +483,10 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
     y=x and h=f work in place."""
     import torch
     index = _device_of(x, "x")
+    if stream is not None:
+        with _given_stream(stream, index):
+            return norm_gate_residual(x, f, post_weight, gate, pre_weight, residual_scale, eps, rows_per_gate, y, h,
+                                      block_dim)
     if x.dim() != 2:
         raise AfirHipError("norm_gate_residual: x must have two dimensions")
     dtype = x.dtype
@@ -498,10 +509,12 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
         _dense(pre_weight, (n,), dtype, index, "pre_weight")
         if h is None:
             h = torch.empty(shape, dtype=dtype, device=x.device)
+        elif h is y:
+            raise AfirHipError("norm_gate_residual: y and h are two results")
         ld_h = _rows(h, shape, dtype, index, "h")
     elif h is not None:
         raise AfirHipError("norm_gate_residual: h needs pre_weight")
-    _launch_on(index, "afir_hip_launch_norm_gate_residual", block_dim, stream,
+    _launch_on(index, "afir_hip_launch_norm_gate_residual", block_dim,
                _PACK11(m, n, rows_per_gate, ld_x, ld_f, ld_gate, ld_y, ld_h, f32_bits(residual_scale), f32_bits(eps), kind),
                None, x, f, post_weight, gate, pre_weight, y, h)
     return (x if f is None else y), h
@@ -514,6 +527,10 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     zero.  dh, pre_weight None: the call had no h (y is not read then)."""
     import torch
     index = _device_of(y, "y")
+    if stream is not None:
+        with _given_stream(stream, index):
+            return norm_gate_residual_backward(dy, dh, y, f, post_weight, gate, pre_weight, residual_scale, eps,
+                                               rows_per_gate, block_dim)
     if y.dim() != 2:
         raise AfirHipError("norm_gate_residual_backward: y must have two dimensions")
     dev, dtype = y.device, y.dtype
@@ -551,8 +568,8 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     dx = torch.empty(shape, dtype=dtype, device=dev)
     tiling = _PACK13(m, n, rows_per_gate, ld_dy, ld_dh, ld_y, ld_f, ld_gate, n, n,
                      f32_bits(residual_scale), f32_bits(eps), kind)
-    ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, y, stream)
-    _launch_on(index, "afir_hip_launch_norm_gate_residual_backward", block_dim, stream, tiling, ws.data_ptr(),
+    ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, y)
+    _launch_on(index, "afir_hip_launch_norm_gate_residual_backward", block_dim, tiling, ws.data_ptr(),
                dy, dh, None if dh is None else y, f, post_weight, gate, pre_weight, dx, df, dpost, dgate, dpre)
     return dx, df, dpost, dgate, dpre
 

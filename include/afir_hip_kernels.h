@@ -185,8 +185,8 @@ uint32_t afir_hip_launch_mxfp4_quantize(uint32_t block_dim, void *stream, void *
  * (v_mfma_scale_f32_16x16x128_f8f6f4).  The scale byte 255 makes every number
  * that its block enters a NaN.  workspace: NULL, or a device buffer on a
  * 16-byte boundary of afir_hip_mxfp4_matmul_workspace_bytes(tiling) bytes,
- * which lets large products run on a faster kernel (0 bytes: none would help,
- * on the current device); a launch leaves nothing in
+ * which lets large products run on a faster kernel (0: they run on it without);
+ * a launch leaves nothing in
  * it that a later one reads, but launches that may overlap need one each.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (K); int64 dim_arg2_0 (N);
  *              int64 alpha_f32_bits; int64 elem_type }                         */

@@ -258,6 +258,54 @@ def test_matmul_scales_at_their_ends(H):
     B.close(got, want, size, "f32", k // 32 + 10)
 
 
+@pytest.mark.parametrize("m,n,k", [(4100, 4200, 1056), (260, 8300, 608), (40, 300, 1184), (300, 200, 640)])
+def test_matmul_of_many_rows_keeps_nan_and_scales_at_their_ends(H, m, n, k):
+    # in rows, columns and the last blocks of both operands: on tiles (the first two) and on a workgroup per tile
+    rng = np.random.default_rng(5)
+    (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
+    asc[:], bsc[:] = 0, 254
+    asc[:, ::2], bsc[:, ::2] = 250, 4
+    asc[m - 1, -1] = asc[2, -4] = 255
+    bsc[7, 0] = bsc[n - 2, -9] = 255
+    want, size = O.matmul(O.decode(ac, asc), O.decode(bc, bsc), None, 1.0)
+    dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
+    got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2], dev[3].view(torch.float8_e8m0fnu),
+                                       alpha=1.0, out_dtype=torch.float32)
+    lost = np.zeros((m, n), dtype=bool)
+    lost[m - 1] = lost[2] = lost[:, 7] = lost[:, n - 2] = True
+    assert np.array_equal(np.isnan(got.cpu().numpy()), lost)
+    keep = torch.from_numpy(~lost).cuda()
+    B.close(got[keep], want[~lost], size[~lost], "f32", k // 32 + 10)
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("axis", [1, 0])
+def test_quantize_in_place(H, kind, axis):
+    x = torch.randn(170, 300, device="cuda").to(B.TYPES[kind])
+    want = H.mxfp4_quantize(x, axis=axis, return_values=True)
+    got = H.mxfp4_quantize(x, axis=axis, values=x)
+    assert got[2] is x
+    for a, b in zip(got, want):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def test_results_on_a_given_stream_come_from_its_memory(H):
+    # memory freed on the current stream may still be written by what runs there
+    x = torch.randn(256, 2048, device="cuda").bfloat16()
+    (qa, sa), (qb, sb) = H.mxfp4_quantize(x), H.mxfp4_quantize(x[:72].contiguous())
+    want = H.mxfp4_matmul_add_leakyrelu(qa, sa, qb, sb)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    freed = [torch.empty_like(t) for t in (qa, sa, want)]
+    places = {t.data_ptr() for t in freed}
+    del freed
+    codes, scales = H.mxfp4_quantize(x, stream=side.cuda_stream)
+    got = H.mxfp4_matmul_add_leakyrelu(codes, scales, qb, sb, stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(codes, qa) and torch.equal(got, want)
+    assert not places & {t.data_ptr() for t in (codes, scales, got)}
+
+
 def test_matmul_refuses(H):
     u8 = dict(dtype=torch.uint8, device="cuda")
     a, b = torch.zeros(4, 32, **u8), torch.zeros(8, 32, **u8)

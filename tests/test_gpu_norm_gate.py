@@ -214,6 +214,13 @@ def test_gate_of_one_dimension(H):
     assert grads[3].shape == (96,) and torch.equal(grads[3], backward(H, v, y, 12)[3][0])
 
 
+def test_two_results_in_one_tensor_are_refused(H):
+    v = inputs(4, 64, 1, "f32", 20)
+    t = torch.empty(4, 64, device="cuda")
+    with pytest.raises(H.AfirHipError, match="two results"):
+        H.norm_gate_residual(v["x"], v["f"], v["post_weight"], v["gate"], v["pre_weight"], y=t, h=t)
+
+
 def test_refusals(H):
     v = inputs(8, 64, 2, "bf16", 16)
     x, f, w, gate = v["x"], v["f"], v["post_weight"], v["gate"]
