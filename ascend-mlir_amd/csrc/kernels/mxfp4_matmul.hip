@@ -26,7 +26,6 @@ __device__ __forceinline__ void finish_one(const MxOperands &p, int m, int n, fl
 // 8192 x 8192).  The eight partial sums meet in LDS and are added in a fixed order.
 // One row: 9.0 us at 8192 x 8192 (4.0 TB/s; the bytes alone take 7.3 as a large copy moves them), 3.5 at
 // 4096 x 4096; 16 rows at 8192 x 8192 9.7.
-// Also products with K below 256 (MT = 4 above 16 rows).
 constexpr int kRowsWaves = 8;
 
 // 16 rows' codes and scales of one step
@@ -53,8 +52,8 @@ struct RowsPiece {
 };
 
 template <int MT, int NT, int KIND>
-__global__ __launch_bounds__(kRowsWaves * 64, MT == 1 ? 4 : 2) void mxfp4_matmul_rows(MxOperands p, int tiles_n,
-                                                                                      int chunks_m, int blocks) {
+__global__ __launch_bounds__(kRowsWaves * 64, 4) void mxfp4_matmul_rows(MxOperands p, int tiles_n, int chunks_m,
+                                                                        int blocks) {
   constexpr int kCols = 16 * NT, kRows = 16 * MT;
   __shared__ f32x4 part[kRowsWaves][kRows * kCols / 4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, g = lane >> 4;
@@ -136,7 +135,63 @@ LaunchStatus rows_launch(const MxOperands &p, uint32_t block_dim, hipStream_t st
   return after_launch();
 }
 
-// A tile per workgroup up to 64 rows (9.2 us against 15.8 on the kernel above at 48 x 8200 x 4096), and while
+// K below 256 (or out of the other kernels' range): a wavefront takes the blocks of its TM * 16 rows of A and
+// TN * 16 of B straight into registers, a slice of eight at a time.  Such a product is bound by its output:
+// 8192 x 8192 x 64 into bfloat16 38 us (3.5 TB/s of output), 4096 x 4096 x 128 12.7 (102 on the kernel above).
+template <int TM, int TN, int KIND>
+__global__ __launch_bounds__(256) void mxfp4_matmul_direct(MxOperands p, int tiles_m, int tiles_n) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, g = lane >> 4;
+  for (int tile = blockIdx.x; tile < tiles_m * tiles_n; tile += gridDim.x) {
+    int tm, tn;
+    map_tile(tile, tiles_m, tiles_n, tm, tn);
+    const int m0 = (tm * 2 + wave / 2) * TM * 16, n0 = (tn * 2 + wave % 2) * TN * 16;
+    f32x4 acc[TM][TN];
+    start_from_bias<KIND>(p, n0, acc);
+    // rows past the end repeat the last one; blocks past it are zeros at scale 1
+    auto load = [&](const unsigned char *codes, const uint8_t *scales, int64_t row, int block, u32x4 &w, uint32_t &s) {
+      const bool there = block < p.kb;
+      const int64_t at = row * p.kb + block;
+      w = there ? *reinterpret_cast<const u32x4 *>(codes + at * kMxBlockBytes) : u32x4{0, 0, 0, 0};
+      s = there ? scales[at] : 127u;
+    };
+    for (int block = g; block - g < p.kb; block += kMxSliceBlocks) {
+      u32x4 a[2][TM], b[2][TN];
+      uint32_t sa[2][TM], sb[2][TN];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int row = n0 + j * 16 + li;
+          load(p.b, p.b_scales, row < p.n ? row : p.n - 1, block + 4 * h, b[h][j], sb[h][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int row = m0 + i * 16 + li;
+          load(p.a, p.a_scales, row < p.m ? row : p.m - 1, block + 4 * h, a[h][i], sa[h][i]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int i = 0; i < TM; ++i) acc[i][j] = mfma_fp4<0, 0>(b[h][j], a[h][i], acc[i][j], sb[h][j], sa[h][i]);
+    }
+    store_outputs<KIND>(p, m0, n0, acc);
+  }
+}
+
+template <int TM, int TN, int KIND>
+LaunchStatus direct_launch(const MxOperands &p, uint32_t block_dim, hipStream_t stream) {
+  const int tiles_m = (p.m + 32 * TM - 1) / (32 * TM), tiles_n = (p.n + 32 * TN - 1) / (32 * TN);
+  const int64_t blocks = (int64_t)tiles_m * tiles_n;
+  if (blocks > 0x7fffffff) return invalid("mxfp4_matmul: too many output tiles");
+  AFIR_LAUNCH("mxfp4_matmul_direct", (mxfp4_matmul_direct<TM, TN, KIND>), dim3(block_dim ? block_dim : (unsigned)blocks),
+              dim3(256), 0, stream, p, tiles_m, tiles_n);
+  return after_launch();
+}
+
+// A tile per workgroup up to 64 rows (9.2 us against 15.8 on the kernel of few rows at 48 x 8200 x 4096), and while
 // each compute unit gets at most one of 128 x 128 (512 x 8192 x 8192: 27 us, 28 on tiles in turn); beyond that
 // tiles in turn (1024 x 8192 x 8192: 45 us against 55).
 bool one_tile_each(const MxOperands &p) {
@@ -153,7 +208,11 @@ LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hi
   if (one_tile_each(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
   if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
   if (mxfp4_ring_supported(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
-  return rows_launch<4, 2, KIND>(p, block_dim, stream);
+  if (p.n > kMxMaxColumns) return rows_launch<1, 2, KIND>(p, block_dim, stream);
+  // (tiles of 64 x 64 while 128 x 128 ones would not fill the chip twice: 100 x 100 x 100 3.3 us against 5.9, but
+  // 4096 x 4096 x 224 16.6 against 13.8)
+  if ((int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128) >= 2 * device_cus()) return direct_launch<4, 4, KIND>(p, block_dim, stream);
+  return direct_launch<2, 2, KIND>(p, block_dim, stream);
 }
 
 }  // namespace

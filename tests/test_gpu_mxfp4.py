@@ -177,10 +177,10 @@ def test_matmul_on_few_workgroups(H, m, n, k):
     ("bf16", 4096, 4352, 608, 7), ("bf16", 4100, 4090, 256, 0), ("f16", 4300, 4100, 4384, 100), ("bf16", 4352, 4096, 512, 0), ("f32", 4129, 4353, 1312, 200)])
 def test_matmul_on_tiles(H, kind, m, n, k, blocks):
     check_matmul(H, m, n, k, kind, block_dim=blocks)
-    # the tiled kernels take whole lines of 256 numbers: shallower products stay on the kernel of few rows, and
-    # few tiles go to the kernel with a workgroup per tile
+    # the tiled kernels take whole lines of 256 numbers, shallower products have a kernel of their own, and few
+    # tiles go to the kernel with a workgroup per tile
     few = -(-m // 128) * -(-n // 128) <= 256
-    assert H.last_launch()["kernel"] == ("mxfp4_matmul_rows" if k <= 224 else
+    assert H.last_launch()["kernel"] == ("mxfp4_matmul_direct" if k <= 224 else
                                          "mxfp4_matmul_ring" if few else "mxfp4_matmul_tiles")
 
 
@@ -205,6 +205,15 @@ def test_matmul_on_tiles(H, kind, m, n, k, blocks):
 def test_matmul_with_a_workgroup_per_tile(H, kind, m, n, k, blocks):
     check_matmul(H, m, n, k, kind, block_dim=blocks)
     assert H.last_launch()["kernel"] == "mxfp4_matmul_ring"
+    check_matmul(H, m, n, k, kind, bias=False, alpha=1.0, seed=1)
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("m,n,k,blocks", [(17, 300, 1, 0), (17, 1, 31, 0), (40, 33, 70, 0), (64, 64, 64, 0), (129, 127, 128, 3),
+                                          (70, 2000, 160, 0), (1000, 1031, 224, 0), (3000, 3010, 97, 0), (4096, 2056, 33, 40)])
+def test_matmul_of_little_depth(H, kind, m, n, k, blocks):
+    check_matmul(H, m, n, k, kind, block_dim=blocks)
+    assert H.last_launch()["kernel"] == "mxfp4_matmul_direct"
     check_matmul(H, m, n, k, kind, bias=False, alpha=1.0, seed=1)
 
 
@@ -258,15 +267,15 @@ def test_matmul_scales_at_their_ends(H):
     B.close(got, want, size, "f32", k // 32 + 10)
 
 
-@pytest.mark.parametrize("m,n,k", [(4100, 4200, 1056), (260, 8300, 608), (40, 300, 1184), (300, 200, 640)])
+@pytest.mark.parametrize("m,n,k", [(4100, 4200, 1056), (260, 8300, 608), (40, 300, 1184), (300, 200, 640), (90, 70, 192), (4100, 4200, 160)])
 def test_matmul_of_many_rows_keeps_nan_and_scales_at_their_ends(H, m, n, k):
-    # in rows, columns and the last blocks of both operands: on tiles (the first two) and on a workgroup per tile
+    # in rows, columns and blocks of both operands: on tiles (the first two), on a workgroup per tile, of little depth
     rng = np.random.default_rng(5)
     (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
     asc[:], bsc[:] = 0, 254
     asc[:, ::2], bsc[:, ::2] = 250, 4
     asc[m - 1, -1] = asc[2, -4] = 255
-    bsc[7, 0] = bsc[n - 2, -9] = 255
+    bsc[7, 0] = bsc[n - 2, max(-9, -bsc.shape[1])] = 255
     want, size = O.matmul(O.decode(ac, asc), O.decode(bc, bsc), None, 1.0)
     dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
     got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2], dev[3].view(torch.float8_e8m0fnu),
