@@ -24,7 +24,7 @@ __device__ __forceinline__ void finish_one(const MxOperands &p, int m, int n, fl
 // Everything of a step is requested before the first product; two workgroups on a compute unit cover the
 // rest (requesting the next step ahead as well gained nothing: 9.3 against 9.0 us for one row at
 // 8192 x 8192).  The eight partial sums meet in LDS and are added in a fixed order.
-// One row: 9.0 us at 8192 x 8192 (4.0 TB/s; the bytes alone take 7.3 as a large copy moves them), 3.5 at
+// One row: 9.0 us at 8192 x 8192 (4.0 TB/s; the bytes alone take 7.3 as a large copy moves them), 3.8 at
 // 4096 x 4096; 16 rows at 8192 x 8192 9.7.
 constexpr int kRowsWaves = 8;
 
@@ -51,10 +51,10 @@ struct RowsPiece {
   }
 };
 
-template <int MT, int NT, int KIND>
+template <int NT, int KIND>
 __global__ __launch_bounds__(kRowsWaves * 64, 4) void mxfp4_matmul_rows(MxOperands p, int tiles_n, int chunks_m,
                                                                         int blocks) {
-  constexpr int kCols = 16 * NT, kRows = 16 * MT;
+  constexpr int kCols = 16 * NT, kRows = 16;
   __shared__ f32x4 part[kRowsWaves][kRows * kCols / 4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, g = lane >> 4;
   const int shift = 8 * g;
@@ -65,29 +65,20 @@ __global__ __launch_bounds__(kRowsWaves * 64, 4) void mxfp4_matmul_rows(MxOperan
     if (tile_n >= tiles_n) continue;
     const int n0 = tile_n * kCols;
     // rows past the end repeat the last one; what they give is not stored
-    int64_t row_a[MT], row_b[NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) row_a[i] = m0 + i * 16 + li < p.m ? m0 + i * 16 + li : p.m - 1;
+    const int64_t row_a = m0 + li < p.m ? m0 + li : p.m - 1;
+    int64_t row_b[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) row_b[j] = n0 + j * 16 + li < p.n ? n0 + j * 16 + li : p.n - 1;
-    f32x4 acc[MT][NT];
+    f32x4 acc[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    RowsPiece a[MT], b[NT];
+    for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    RowsPiece a, b[NT];
     auto multiply = [&]() {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t sb[NT];
+        const uint32_t sa = a.s[c] >> shift;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sb[j] = b[j].s[c] >> shift;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint32_t sa = a[i].s[c] >> shift;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_fp4<0, 0>(b[j].w[c], a[i].w[c], acc[i][j], sb[j], sa);
-        }
+        for (int j = 0; j < NT; ++j) acc[j] = mfma_fp4<0, 0>(b[j].w[c], a.w[c], acc[j], b[j].s[c] >> shift, sa);
       }
     };
     const int whole = p.kb / 16;   // steps of 16 blocks
@@ -95,22 +86,18 @@ __global__ __launch_bounds__(kRowsWaves * 64, 4) void mxfp4_matmul_rows(MxOperan
     for (; step < whole; step += kRowsWaves) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) b[j].load(p.b, p.b_scales, row_b[j], p.kb, step, g);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i].load(p.a, p.a_scales, row_a[i], p.kb, step, g);
+      a.load(p.a, p.a_scales, row_a, p.kb, step, g);
       multiply();
     }
     if (step == whole && whole * 16 < p.kb) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) b[j].load_tail(p.b, p.b_scales, row_b[j], p.kb, step, g);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i].load_tail(p.a, p.a_scales, row_a[i], p.kb, step, g);
+      a.load_tail(p.a, p.a_scales, row_a, p.kb, step, g);
       multiply();
     }
-    // part[wave]: row-major [kRows][kCols]; lane: row i * 16 + li, columns j * 16 + 4 g ..
+    // part[wave]: row-major [kRows][kCols]; lane: row li, columns j * 16 + 4 g ..
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) part[wave][((i * 16 + li) * kCols + j * 16 + 4 * g) / 4] = acc[i][j];
+    for (int j = 0; j < NT; ++j) part[wave][(li * kCols + j * 16 + 4 * g) / 4] = acc[j];
     __syncthreads();
     for (int e = t; e < kRows * kCols; e += kRowsWaves * 64) {
       const int m = m0 + e / kCols, n = n0 + e % kCols;
@@ -125,12 +112,12 @@ __global__ __launch_bounds__(kRowsWaves * 64, 4) void mxfp4_matmul_rows(MxOperan
   }
 }
 
-template <int MT, int NT, int KIND>
+template <int NT, int KIND>
 LaunchStatus rows_launch(const MxOperands &p, uint32_t block_dim, hipStream_t stream) {
-  const int tiles_n = (p.n + 16 * NT - 1) / (16 * NT), chunks_m = (p.m + 16 * MT - 1) / (16 * MT);
+  const int tiles_n = (p.n + 16 * NT - 1) / (16 * NT), chunks_m = (p.m + 15) / 16;
   const int64_t blocks = (int64_t)((tiles_n + kNumXCD - 1) / kNumXCD) * kNumXCD * chunks_m;
   if (blocks > 0x7fffffff) return invalid("mxfp4_matmul: too many output tiles");
-  AFIR_LAUNCH("mxfp4_matmul_rows", (mxfp4_matmul_rows<MT, NT, KIND>), dim3(block_dim ? block_dim : (unsigned)blocks),
+  AFIR_LAUNCH("mxfp4_matmul_rows", (mxfp4_matmul_rows<NT, KIND>), dim3(block_dim ? block_dim : (unsigned)blocks),
               dim3(kRowsWaves * 64), 0, stream, p, tiles_n, chunks_m, (int)blocks);
   return after_launch();
 }
@@ -202,13 +189,13 @@ bool one_tile_each(const MxOperands &p) {
 template <int KIND>
 LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hipStream_t stream) {
   // Up to 16 rows; 16 columns a workgroup where that gives no compute unit a second one (4096 x 4096, one row:
-  // 3.5 us against 4.8 with 32; 8192 x 8192, 16 rows: 11.8 against 9.7).
-  if (p.m <= 16 && p.n <= 16 * device_cus()) return rows_launch<1, 1, KIND>(p, block_dim, stream);
-  if (p.m <= 16) return rows_launch<1, 2, KIND>(p, block_dim, stream);
+  // 3.8 us against 4.8 with 32; 8192 x 8192, 16 rows: 11.8 against 9.6).
+  if (p.m <= 16 && p.n <= 16 * device_cus()) return rows_launch<1, KIND>(p, block_dim, stream);
+  if (p.m <= 16) return rows_launch<2, KIND>(p, block_dim, stream);
   if (one_tile_each(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
   if (workspace && mxfp4_dma_supported(p)) return launch_mxfp4_dma(p, KIND, workspace, block_dim, stream);
   if (mxfp4_ring_supported(p)) return launch_mxfp4_ring(p, KIND, block_dim, stream);
-  if (p.n > kMxMaxColumns) return rows_launch<1, 2, KIND>(p, block_dim, stream);
+  if (p.n > kMxMaxColumns) return rows_launch<2, KIND>(p, block_dim, stream);
   // (tiles of 64 x 64 while 128 x 128 ones would not fill the chip twice: 100 x 100 x 100 3.3 us against 5.9, but
   // 4096 x 4096 x 224 16.6 against 13.8)
   if ((int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128) >= 2 * device_cus()) return direct_launch<4, 4, KIND>(p, block_dim, stream);

@@ -222,27 +222,35 @@ LaunchStatus forward(const NormGateArgs &p, uint32_t block_dim, hipStream_t stre
 // mean(a yn) and both rstd need one round of row sums, mean(b fn) a second one; nothing is kept
 // from the forward pass but y.
 //
-// The column sums: a workgroup walks a stretch of rows and keeps its share of a row's columns in
-// registers, then writes one row of float32 partial sums, which a second kernel adds in a fixed
-// order.  A stretch never straddles two gate rows unless it covers each of them whole, so either
-// the gate is one row throughout (kOneGate: the partial sum is that of t fn, which serves dgate
-// and, weighted with the gate, dpost_weight), or dgate's rows are finished within the workgroup.
+// The column sums: the wavefronts of a row walk a stretch of rows and keep their share of its columns
+// in registers.  A workgroup has eight wavefronts where a row has fewer, adds its stretches' sums in LDS
+// and writes one row of float32 partial sums, which a second kernel adds; all in a fixed order.  A
+// stretch never straddles two gate rows unless it covers each of them whole, so either the gate is
+// one row throughout a workgroup (kOneGate: the partial sum is that of t fn, which serves dgate and,
+// weighted with the gate, dpost_weight), or dgate's rows are finished within the stretch.
+// (bf16 8192 x 32: 20 us; with a partial row per stretch 48, most of it their sum.)
+constexpr int groups_of(int waves) { return waves < 8 ? 8 / waves : 1; }   // stretches of a workgroup
 struct Stretches {       // stretch i: rows from (i / per_span) * span + (i % per_span) * rows
   uint32_t span;         // rows of one gate row, or of several whole ones
-  uint32_t per_span, rows, count;
+  uint32_t per_span, rows, count;   // (per_span and count: whole workgroups of stretches)
   bool one_gate;
 };
 
-inline Stretches plan_stretches(int64_t m, int64_t rows_per_gate, bool gate, int64_t workgroups) {
-  const int64_t rows = (m + workgroups - 1) / workgroups, per_gate = gate && rows_per_gate < m ? rows_per_gate : m;
-  const bool whole = gate && per_gate <= rows;   // gate rows, as many as fit
-  const int64_t span = whole ? rows / per_gate * per_gate : per_gate, per_span = whole ? 1 : (per_gate + rows - 1) / rows;
+inline Stretches plan_stretches(int64_t m, int64_t rows_per_gate, bool gate, int64_t stretches, int groups) {
+  const int64_t rows = (m + stretches - 1) / stretches, per_gate = gate && rows_per_gate < m ? rows_per_gate : m;
+  // Whole gate rows, as many as fit; or one longer than `rows`, where splitting it over a workgroup's stretches
+  // would leave many of them idle (bf16 8192 x 256, 3 rows to a gate: 27 us against 75; 16 rows: 68 against 24).
+  const bool whole = gate && per_gate <= rows * (groups + 1) / 2;
+  const int64_t span = whole && per_gate < rows ? rows / per_gate * per_gate : per_gate;
+  int64_t per_span = whole ? 1 : (per_gate + rows - 1) / rows, count = (m + span - 1) / span;
   Stretches s;
   s.one_gate = !whole || per_gate == m;
+  if (s.one_gate) per_span = (per_span + groups - 1) / groups * groups;
+  count = (count * per_span + groups - 1) / groups * groups;
   s.span = (uint32_t)span;
   s.per_span = (uint32_t)per_span;
   s.rows = (uint32_t)((span + per_span - 1) / per_span);
-  s.count = (uint32_t)((m + span - 1) / span * per_span);
+  s.count = (uint32_t)count;
   return s;
 }
 
@@ -259,17 +267,24 @@ __device__ __forceinline__ void store_sums(float *row, uint32_t e, uint32_t n, c
 }
 
 template <int KIND, int WAVES, int ITEMS, bool kOneGate>
-__global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGradArgs p, Stretches s) {
+__global__ __launch_bounds__(WAVES * groups_of(WAVES) * 64, 4) void norm_gate_backward(NormGateGradArgs p, Stretches s) {
   constexpr int V = Elem<KIND>::kPer16, kLanes = WAVES * 64;
+  constexpr int kGroups = groups_of(WAVES);
   constexpr bool kAhead = ITEMS == 1;
-  __shared__ __align__(16) float lds[2 * WAVES * 4];
-  const int lane = threadIdx.x, wave = lane >> 6;
+  // rows of several wavefronts meet at barriers, so stretches of one workgroup take the same number of steps
+  constexpr bool kMayIdle = kGroups > 1 && WAVES > 1;
+  __shared__ __align__(16) float sums_lds[kGroups][2 * WAVES * 4];
+  __shared__ f32x4 joined[kGroups > 1 ? kGroups - 1 : 1][kGroups > 1 ? V / 4 : 1][kLanes];
+  const int lane = threadIdx.x % kLanes, wave = lane >> 6;
+  const int group = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);   // (a scalar, like its rows)
+  float *const lds = sums_lds[group];
   const uint32_t n = (uint32_t)p.n;
   Piece<KIND, ITEMS> post, pre;
   if (!kOneGate && p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
   if (p.dh) load_row<KIND, kLanes, ITEMS>(p.pre_weight, 0, lane, n, pre);
   int turn = 0;
-  for (uint32_t stretch = blockIdx.x; stretch < s.count; stretch += gridDim.x) {
+  for (uint32_t place = blockIdx.x; place < s.count / kGroups; place += gridDim.x) {
+    const uint32_t stretch = place * kGroups + group;
     const int64_t first = (int64_t)(stretch / s.per_span) * s.span, r0 = first + (int64_t)(stretch % s.per_span) * s.rows;
     int64_t r1 = r0 + s.rows < first + s.span ? r0 + s.rows : first + s.span;
     r1 = r1 < p.m ? r1 : p.m;
@@ -282,6 +297,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
         if constexpr (!kOneGate) acc_gate[i][j] = 0.f;
       }
     Piece<KIND, ITEMS> dy, dh, y, f, gate;
+    if constexpr (kMayIdle) dy = dh = y = f = gate = Piece<KIND, ITEMS>{};
     auto fetch = [&](int64_t r) {
       if (p.dy) load_row<KIND, kLanes, ITEMS>(p.dy, r * p.ld_dy, lane, n, dy);
       if (p.dh) {
@@ -295,7 +311,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
     };
     if (r0 < r1) {
       if (kOneGate && p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
-      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(r0, p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(first, p.rows_per_gate) * p.ld_gate, lane, n, gate);
       fetch(r0);
     }
     // gate post_weight: held through the stretch where it is one row and there are registers for it
@@ -325,7 +341,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] *= vw[j];
     };
-    for (int64_t row = r0; row < r1; ++row) {
+    const int64_t end = kMayIdle ? r0 + s.rows : r1;
+    for (int64_t row = r0; row < end; ++row) {
+      const bool active = !kMayIdle || row < r1;
       float sums[3] = {0.f, 0.f, 0.f};   // y^2, a y, f^2
       float a[V], t[ITEMS][V];   // (a stays where there are registers, or is formed anew)
 #pragma unroll
@@ -351,6 +369,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
       const float ry = rstd_of(sums[0], p.inv_n, p.eps), rf = rstd_of(sums[2], p.inv_n, p.eps);
       const float my = ry * sums[1] * p.inv_n;   // mean(a yn)
       float dot[1] = {0.f};                      // b f
+      if (active) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         if (p.dy) Elem<KIND>::unpack(dy.w[i], t[i]);
@@ -387,6 +406,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
           }
         }
       }
+      }
       // the next row is requested here, ahead of this row's stores and second round of sums; rows of
       // several pieces per lane have no registers for two rows and request theirs when they are done
       const Piece<KIND, ITEMS> f_here = f, gate_here = gate;
@@ -396,7 +416,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = p.residual_scale * t[i][j];
-        store_item<KIND, kLanes>(p.dx, row * p.ld_dx, (uint32_t)(lane + i * kLanes) * V, n, o);
+        if (active) store_item<KIND, kLanes>(p.dx, row * p.ld_dx, (uint32_t)(lane + i * kLanes) * V, n, o);
       }
       if (p.f) {
         row_sums<WAVES>(dot, lds, turn, wave);
@@ -408,10 +428,10 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
           weight_row(i, gate_here, vw);
 #pragma unroll
           for (int j = 0; j < V; ++j) o[j] = rf * (t[i][j] * vw[j] - vf[j] * rf * mf);
-          store_item<KIND, kLanes>(p.df, row * p.ld_df, (uint32_t)(lane + i * kLanes) * V, n, o);
+          if (active) store_item<KIND, kLanes>(p.df, row * p.ld_df, (uint32_t)(lane + i * kLanes) * V, n, o);
         }
         if constexpr (!kOneGate) {
-          if ((uint32_t)(row + 1) % (uint32_t)p.rows_per_gate == 0 || row + 1 == p.m) {
+          if (active && ((uint32_t)(row + 1) % (uint32_t)p.rows_per_gate == 0 || row + 1 == p.m)) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
               float o[V], vw[V];
@@ -428,13 +448,31 @@ __global__ __launch_bounds__(WAVES * 64, 4) void norm_gate_backward(NormGateGrad
       }
       if (!kAhead && row + 1 < r1) fetch(row + 1);
     }
-    float *const part_post = p.partial + (int64_t)stretch * p.n, *const part_pre = p.partial + ((int64_t)s.count + stretch) * p.n;
+    if constexpr (kGroups > 1) {
+      auto join = [&](float (&acc)[V]) {
+        __syncthreads();
+        if (group > 0)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const uint32_t e = (uint32_t)(lane + i * kLanes) * V;
-      if (p.f) store_sums(part_post, e, n, acc_post[i]);
-      if (p.dh) store_sums(part_pre, e, n, acc_pre[i]);
+          for (int j = 0; j < V; j += 4) joined[group - 1][j / 4][lane] = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+          for (int other = 0; other < kGroups - 1; ++other)
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += joined[other][j / 4][lane][j % 4];
+      };
+      if (p.f) join(acc_post[0]);
+      if (p.dh) join(acc_pre[0]);
     }
+    float *const part_post = p.partial + (int64_t)place * p.n;
+    float *const part_pre = p.partial + ((int64_t)(s.count / kGroups) + place) * p.n;
+    if (group == 0)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t e = (uint32_t)(lane + i * kLanes) * V;
+        if (p.f) store_sums(part_post, e, n, acc_post[i]);
+        if (p.dh) store_sums(part_pre, e, n, acc_pre[i]);
+      }
   }
 }
 
@@ -515,25 +553,28 @@ inline RowShape backward_shape(int64_t n, int elem_kind) {
 }
 inline Stretches backward_stretches(int64_t m, int64_t n, int64_t rows_per_gate, bool gate, int elem_kind) {
   const int waves = backward_shape(n, elem_kind).waves;
-  return plan_stretches(m, rows_per_gate, gate, (int64_t)device_cus() * (waves <= 8 ? 16 / waves : 1));
+  return plan_stretches(m, rows_per_gate, gate, (int64_t)device_cus() * (waves <= 8 ? 16 / waves : 1), groups_of(waves));
 }
 
 template <int KIND, int WAVES, int ITEMS>
 LaunchStatus backward_launch(const NormGateGradArgs &p, const Stretches &s, uint32_t block_dim, hipStream_t stream) {
-  const int64_t most = (int64_t)1 << 20;
-  const int64_t blocks = block_dim ? block_dim : s.count < most ? s.count : most;
+  constexpr int kGroups = groups_of(WAVES);
+  const int64_t most = (int64_t)1 << 20, all = s.count / kGroups, blocks = block_dim ? block_dim : all < most ? all : most;
   if (s.one_gate)
     AFIR_LAUNCH("norm_gate_backward", (norm_gate_backward<KIND, WAVES, ITEMS, true>), dim3((unsigned)blocks),
-                dim3(WAVES * 64), 0, stream, p, s);
+                dim3(WAVES * kGroups * 64), 0, stream, p, s);
   else
     AFIR_LAUNCH("norm_gate_backward", (norm_gate_backward<KIND, WAVES, ITEMS, false>), dim3((unsigned)blocks),
-                dim3(WAVES * 64), 0, stream, p, s);
+                dim3(WAVES * kGroups * 64), 0, stream, p, s);
   const LaunchStatus st = after_launch();
   if (st.code) return st;
   const int64_t column_tiles = (p.n + kJoinColumns - 1) / kJoinColumns;
+  Stretches partial = s;   // in rows of partial sums
+  partial.count /= kGroups;
+  if (s.one_gate) partial.per_span /= kGroups;
   const int64_t gates = s.one_gate && p.f && p.gate ? (p.m + p.rows_per_gate - 1) / p.rows_per_gate : 0;
   AFIR_LAUNCH("norm_gate_join", (norm_gate_join<KIND>), dim3((unsigned)column_tiles, (unsigned)(2 + gates)),
-              dim3(kJoinWaves * 64), 0, stream, p, s, column_tiles);
+              dim3(kJoinWaves * 64), 0, stream, p, partial, column_tiles);
   return after_launch();
 }
 
@@ -586,7 +627,8 @@ LaunchStatus launch_norm_gate_residual(const NormGateArgs &args, int elem_kind, 
 
 size_t norm_gate_backward_workspace(int64_t m, int64_t n, int64_t rows_per_gate, bool gate, int elem_kind) {
   if (m <= 0 || n <= 0 || rows_per_gate < 1) return 0;
-  return (size_t)backward_stretches(m, n, rows_per_gate, gate, elem_kind).count * (size_t)n * 2 * sizeof(float);
+  return (size_t)(backward_stretches(m, n, rows_per_gate, gate, elem_kind).count /
+                  groups_of(backward_shape(n, elem_kind).waves)) * (size_t)n * 2 * sizeof(float);
 }
 
 LaunchStatus launch_norm_gate_residual_backward(const NormGateGradArgs &args, int elem_kind, uint32_t block_dim,

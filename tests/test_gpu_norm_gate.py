@@ -91,6 +91,21 @@ def test_forward_and_backward(H, kind, m, n, rows_per_gate):
     check_backward(v, got[0], backward(H, v, got[0], rows_per_gate), kind, rows_per_gate)
 
 
+@pytest.mark.parametrize("kind,m,n,rows_per_gate", [
+    # rows of one, two and four wavefronts, whose workgroups walk several stretches; gates shorter than a stretch, a
+    # little longer, split over stretches with some left idle, and one for all
+    ("bf16", 8192, 40, 3), ("f32", 8200, 72, 10), ("f16", 8191, 256, 20), ("bf16", 4097, 513, 2), ("f32", 5000, 260, 1),
+    ("f16", 4100, 900, 9), ("bf16", 6001, 600, 700), ("f32", 3000, 1000, 11), ("f16", 2600, 2048, 3), ("bf16", 2100, 1100, 7),
+    ("f32", 2049, 600, 2049), ("bf16", 8192, 64, 0), ("f16", 4099, 33, 4099)])
+def test_gradients_of_many_short_rows(H, kind, m, n, rows_per_gate):
+    v = inputs(m, n, rows_per_gate, kind, m + n)
+    y, _ = forward(H, v, rows_per_gate)
+    got = backward(H, v, y, rows_per_gate)
+    check_backward(v, y, got, kind, rows_per_gate)
+    for a, b in zip(backward(H, v, y, rows_per_gate, block_dim=3), got):
+        assert (a is None and b is None) or torch.equal(a, b)
+
+
 @pytest.mark.parametrize("m,n,rows_per_gate", [(37, 300, 5), (300, 2048, 1), (515, 96, 129)])
 def test_parts_left_out(H, m, n, rows_per_gate):
     kind = "bf16"
