@@ -354,17 +354,24 @@ def _launch_on(index, symbol, block_dim, tiling, workspace, *tensors):
         _check(rc)
 
 
+def _like(t):
+    """A dense tensor of t's shape and type.  (An allocation is a tenth of a call: empty_like takes 1.2 us,
+    new_empty 1.7 and empty with a type and a device 2.2.)"""
+    import torch
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _workspace(query, tiling, like):
     """Scratch of the size that the library asks for, from torch's allocator, which hands it
     out again only to work that follows on the current stream, that of this call."""
-    import torch
     fn = _entries.get(query)
     if fn is None:
         fn = _entries[query] = getattr(load(), query)
     size = fn(tiling)
     if not size:
         return None
-    return torch.empty((size,), dtype=torch.uint8, device=like.device)
+    import torch
+    return like.new_empty((size,), dtype=torch.uint8)
 
 
 _PACK5, _PACK11, _PACK13 = (struct.Struct(f"<{count}q").pack for count in (5, 11, 13))
@@ -394,17 +401,17 @@ def mxfp4_quantize(x, axis=-1, codes=None, scales=None, values=None, return_valu
     k, r = shape if axis == 0 else (shape[1], shape[0])
     kb = (k + 31) // 32
     if codes is None:
-        codes = torch.empty((r, kb * 16), dtype=torch.uint8, device=x.device)
+        codes = x.new_empty((r, kb * 16), dtype=torch.uint8)
     else:
         _dense(codes, (r, kb * 16), torch.uint8, index, "codes")
     if scales is None:
-        scales = torch.empty((r, kb), dtype=torch.float8_e8m0fnu, device=x.device)
+        scales = x.new_empty((r, kb), dtype=torch.float8_e8m0fnu)
     else:
         _dense(scales, (r, kb), torch.float8_e8m0fnu, index, "scales")
     if values is not None:
         _dense(values, shape, dtype, index, "values")
     elif return_values:
-        values = torch.empty(shape, dtype=dtype, device=x.device)
+        values = _like(x)
     _launch_on(index, "afir_hip_launch_mxfp4_quantize", block_dim,
                _PACK5(shape[0], shape[1], ld, 0 if axis == 0 else 1, kind), None, x, codes, scales, values)
     return (codes, scales) if values is None else (codes, scales, values)
@@ -439,7 +446,7 @@ def mxfp4_matmul_add_leakyrelu(a, a_scales, b, b_scales, bias=None, alpha=0.01, 
     if out is None:
         dtype = torch.bfloat16 if out_dtype is None else out_dtype
         kind = _elem_type(dtype, "out")
-        out = torch.empty((m, n), dtype=dtype, device=a.device)
+        out = a.new_empty((m, n), dtype=dtype)
     else:
         dtype = out.dtype if out_dtype is None else out_dtype
         kind = _elem_type(dtype, "out")
@@ -481,7 +488,6 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
     row i // rows_per_gate (None: one gate row for all rows, or one each).  Without f, y is x
     (the norm ahead of the first block); without pre_weight there is no h.  Returns (y, h).
     y=x and h=f work in place."""
-    import torch
     index = _device_of(x, "x")
     if stream is not None:
         with _given_stream(stream, index):
@@ -503,12 +509,12 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
         _dense(post_weight, (n,), dtype, index, "post_weight")
         rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, index)
         if y is None:
-            y = torch.empty(shape, dtype=dtype, device=x.device)
+            y = _like(x)
         ld_y = _rows(y, shape, dtype, index, "y")
     if pre_weight is not None:
         _dense(pre_weight, (n,), dtype, index, "pre_weight")
         if h is None:
-            h = torch.empty(shape, dtype=dtype, device=x.device)
+            h = _like(x)
         elif h is y:
             raise AfirHipError("norm_gate_residual: y and h are two results")
         ld_h = _rows(h, shape, dtype, index, "h")
@@ -525,7 +531,6 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     """The gradients (dx, df, dpost_weight, dgate, dpre_weight) of norm_gate_residual from
     those of its results and the y it returned; None where it had no such input.  dy None:
     zero.  dh, pre_weight None: the call had no h (y is not read then)."""
-    import torch
     index = _device_of(y, "y")
     if stream is not None:
         with _given_stream(stream, index):
@@ -533,7 +538,7 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
                                                rows_per_gate, block_dim)
     if y.dim() != 2:
         raise AfirHipError("norm_gate_residual_backward: y must have two dimensions")
-    dev, dtype = y.device, y.dtype
+    dtype = y.dtype
     kind = _elem_type(dtype, "y")
     m, n = shape = y.shape
     if m == 0 or n == 0:
@@ -552,7 +557,7 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
     if dh is not None:
         ld_dh = _rows(dh, shape, dtype, index, "dh")
         _dense(pre_weight, (n,), dtype, index, "pre_weight")
-        dpre = torch.empty((n,), dtype=dtype, device=dev)
+        dpre = _like(pre_weight)
     if f is None:
         if post_weight is not None or gate is not None:
             raise AfirHipError("norm_gate_residual_backward: post_weight and gate need f")
@@ -561,11 +566,11 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
         ld_f = _rows(f, shape, dtype, index, "f")
         _dense(post_weight, (n,), dtype, index, "post_weight")
         rows_per_gate, ld_gate = _gate_rows(gate, m, n, rows_per_gate, dtype, index)
-        df = torch.empty(shape, dtype=dtype, device=dev)
-        dpost = torch.empty((n,), dtype=dtype, device=dev)
+        df = _like(y)
+        dpost = _like(post_weight)
         if gate is not None:
-            dgate = torch.empty(gate.shape, dtype=dtype, device=dev)
-    dx = torch.empty(shape, dtype=dtype, device=dev)
+            dgate = _like(gate)
+    dx = _like(y)
     tiling = _PACK13(m, n, rows_per_gate, ld_dy, ld_dh, ld_y, ld_f, ld_gate, n, n,
                      f32_bits(residual_scale), f32_bits(eps), kind)
     ws = _workspace("afir_hip_norm_gate_residual_backward_workspace_bytes", tiling, y)

@@ -238,6 +238,16 @@ def test_matmul_without_depth_is_the_bias(H):
     assert not H.mxfp4_matmul_add_leakyrelu(a, s(a), b, s(b)).any()
 
 
+@pytest.mark.parametrize("m", [1, 17, 300])
+def test_matmul_without_depth_for_any_number_of_rows(H, m):
+    a, b = (torch.zeros((r, 0), dtype=torch.uint8, device="cuda") for r in (m, 40))
+    scales = [t.view(torch.float8_e8m0fnu) for t in (a, b)]
+    bias = torch.linspace(-3, 5, 40, device="cuda")
+    got = H.mxfp4_matmul_add_leakyrelu(a, scales[0], b, scales[1], bias, alpha=0.5, out_dtype=torch.float32)
+    assert torch.equal(got, torch.maximum(bias, bias * 0.5).expand(m, 40))
+    assert not H.mxfp4_matmul_add_leakyrelu(a, scales[0], b, scales[1]).any()
+
+
 def test_matmul_keeps_nan_to_the_rows_and_columns_that_hold_it(H):
     rng = np.random.default_rng(3)
     for m, n, k in ((5, 40, 320), (70, 80, 1056)):
