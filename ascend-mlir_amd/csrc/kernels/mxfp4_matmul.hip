@@ -39,7 +39,8 @@ struct RowsPiece {
     s = *reinterpret_cast<const u32x4_any *>(scales + row * kb + step * 16);
   }
   // the blocks past the end: zeros, at scale 1
-  __device__ __forceinline__ void load_tail(const unsigned char *codes, const uint8_t *scales, int64_t row, int kb, int step, int g) {
+  __device__ __forceinline__ void load_tail(const unsigned char *codes, const uint8_t *scales, int64_t row, int kb, int step,
+                                            int g) {
     uint32_t v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -198,7 +199,8 @@ LaunchStatus matmul(const MxOperands &p, void *workspace, uint32_t block_dim, hi
   if (p.n > kMxMaxColumns) return rows_launch<2, KIND>(p, block_dim, stream);
   // (tiles of 64 x 64 while 128 x 128 ones would not fill the chip twice: 100 x 100 x 100 3.3 us against 5.9, but
   // 4096 x 4096 x 224 16.6 against 13.8)
-  if ((int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128) >= 2 * device_cus()) return direct_launch<4, 4, KIND>(p, block_dim, stream);
+  if ((int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128) >= 2 * device_cus())
+    return direct_launch<4, 4, KIND>(p, block_dim, stream);
   return direct_launch<2, 2, KIND>(p, block_dim, stream);
 }
 

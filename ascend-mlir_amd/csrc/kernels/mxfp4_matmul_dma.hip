@@ -256,7 +256,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mxfp4_matmul_tiles(MxOperands 
     if constexpr (R < TM / 4) read8<R * kUnitBytes>(ssa, sa_next[R]);
     else if constexpr (R < kScaleReads) read8<(R - TM / 4) * kUnitBytes>(ssb, sb_next[R - TM / 4]);
     else if constexpr (R == kScaleReads) read_b(ba, b0, std::integral_constant<int, 0>{});
-    else if constexpr (R <= kScaleReads + kHalf) read_a(std::integral_constant<int, 0>{}, aa, a0, std::integral_constant<int, R - kScaleReads - 1>{});
+    else if constexpr (R <= kScaleReads + kHalf)
+      read_a(std::integral_constant<int, 0>{}, aa, a0, std::integral_constant<int, R - kScaleReads - 1>{});
     else read_b(ba, b0, std::integral_constant<int, R - kScaleReads - kHalf>{});
   };
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };

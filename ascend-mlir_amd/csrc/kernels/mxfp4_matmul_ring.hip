@@ -9,8 +9,9 @@
 //
 // The scales of 32 slices (or of fewer, rounded up to a power of two) come first, whole 16-byte pieces
 // swizzled by the row, so that the reads of sixteen rows' eight bytes meet no bank twice.  (Eight bytes a
-// row with every slice took half as many instructions again as the slice itself.)  A last slice that is not whole starts early, so that it ends with the row; the
-// blocks that it repeats get the scale 2^-127 on both sides, and their products vanish in float32.
+// row with every slice took half as many instructions again as the slice itself.)  A last slice that is
+// not whole starts early, so that it ends with the row; the blocks that it repeats get the scale 2^-127 on
+// both sides, and their products vanish in float32.
 //
 // How deep the ring is (3, 4 or 8 slots) measured the same.  What a slice costs is its issue, LDS and
 // barrier time: requesting the next lines between the products took 512 x 8192 x 8192 from 28.3 to 26.1 us;
@@ -230,8 +231,10 @@ mxfp4_matmul_ring(MxOperands p, int slices, ScaleRows how, int tiles_m, int tile
         // the reads over the first 3/4 of the products; the loads over all of them, where no other workgroup
         // on the compute unit fills the time that their issue takes
         static_for<0, 2 * TN>([&](auto x_tag) {
-          constexpr int x = decltype(x_tag)::value, h = x / TN, j = x % TN, parts = 2 * TN * 3 / 4, load_parts = T::kLds > 80 * 1024 ? 2 * TN : 1;
-          if constexpr (x < parts) static_for<kReads * x / parts, kReads *(x + 1) / parts>([&](auto r) { read_one(next, at, r); });
+          constexpr int x = decltype(x_tag)::value, h = x / TN, j = x % TN;
+          constexpr int parts = 2 * TN * 3 / 4, load_parts = T::kLds > 80 * 1024 ? 2 * TN : 1;
+          if constexpr (x < parts)
+            static_for<kReads * x / parts, kReads *(x + 1) / parts>([&](auto r) { read_one(next, at, r); });
           if constexpr (STEADY && x < load_parts)
             static_for<T::kLoads * x / load_parts, T::kLoads *(x + 1) / load_parts>([&](auto q) { load_region(block, free, q); });
           __builtin_amdgcn_sched_barrier(0);
@@ -291,8 +294,8 @@ LaunchStatus ring_launch(const MxOperands &p, uint32_t block_dim, hipStream_t st
   if (blocks > 0x7fffffff) return invalid("mxfp4_matmul: too many output tiles");
   const uintptr_t starts = reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales);
   const ScaleRows how = (starts | (uintptr_t)p.kb) % 16 == 0 ? kPieces : (starts | (uintptr_t)p.kb) % 4 == 0 ? kWords : kBytes;
-  AFIR_LAUNCH("mxfp4_matmul_ring", (mxfp4_matmul_ring<WM, WN, TM, TN, SLOTS, KIND>), dim3(block_dim ? block_dim : (unsigned)blocks),
-              dim3(T::kWaves * 64), 0, stream, p, (p.kb + kMxSliceBlocks - 1) / kMxSliceBlocks, how, tiles_m, tiles_n);
+  AFIR_LAUNCH("mxfp4_matmul_ring", (mxfp4_matmul_ring<WM, WN, TM, TN, SLOTS, KIND>),
+              dim3(block_dim ? block_dim : (unsigned)blocks), dim3(T::kWaves * 64), 0, stream, p, (p.kb + kMxSliceBlocks - 1) / kMxSliceBlocks, how, tiles_m, tiles_n);
   return after_launch();
 }
 

@@ -46,11 +46,8 @@ template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// until at most N LDS reads are outstanding
-template <int N = 0>
 __device__ __forceinline__ void wait_lds() {
-  static_assert(N < 16, "the counter has four bits");
-  asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 template <int OFF>
 __device__ __forceinline__ void read16(uint32_t addr, u32x4 &dst) {

@@ -314,7 +314,8 @@ __global__ __launch_bounds__(WAVES * groups_of(WAVES) * 64, 4) void norm_gate_ba
     };
     if (r0 < r1) {
       if (kOneGate && p.f) load_row<KIND, kLanes, ITEMS>(p.post_weight, 0, lane, n, post);
-      if (kOneGate && p.f && p.gate) load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(first, p.rows_per_gate) * p.ld_gate, lane, n, gate);
+      if (kOneGate && p.f && p.gate)
+        load_row<KIND, kLanes, ITEMS>(p.gate, gate_row(first, p.rows_per_gate) * p.ld_gate, lane, n, gate);
       fetch(r0);
     }
     // gate post_weight: held through the stretch where it is one row and there are registers for it
@@ -374,41 +375,41 @@ __global__ __launch_bounds__(WAVES * groups_of(WAVES) * 64, 4) void norm_gate_ba
       float dot[1] = {0.f};                      // b f
       if (active) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        if (p.dy) Elem<KIND>::unpack(dy.w[i], t[i]);
-        else
+        for (int i = 0; i < ITEMS; ++i) {
+          if (p.dy) Elem<KIND>::unpack(dy.w[i], t[i]);
+          else
 #pragma unroll
-          for (int j = 0; j < V; ++j) t[i][j] = 0.f;
-        if (p.dh) {
-          float vy[V], vd[V];
-          Elem<KIND>::unpack(y.w[i], vy);
-          Elem<KIND>::unpack(dh.w[i], vd);
-          if (ITEMS > 1 || !kOneGate) unpack_a(i, a);
+            for (int j = 0; j < V; ++j) t[i][j] = 0.f;
+          if (p.dh) {
+            float vy[V], vd[V];
+            Elem<KIND>::unpack(y.w[i], vy);
+            Elem<KIND>::unpack(dh.w[i], vd);
+            if (ITEMS > 1 || !kOneGate) unpack_a(i, a);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float yn = vy[j] * ry;
-            t[i][j] += ry * (a[j] - yn * my);
-            acc_pre[i][j] += vd[j] * yn;
+            for (int j = 0; j < V; ++j) {
+              const float yn = vy[j] * ry;
+              t[i][j] += ry * (a[j] - yn * my);
+              acc_pre[i][j] += vd[j] * yn;
+            }
           }
-        }
-        if (p.f) {
-          float vf[V], vg[V], vw[V];
-          Elem<KIND>::unpack(f.w[i], vf);
-          weight_row(i, gate, vw);
-          if (!kOneGate && p.gate) Elem<KIND>::unpack(gate.w[i], vg);
+          if (p.f) {
+            float vf[V], vg[V], vw[V];
+            Elem<KIND>::unpack(f.w[i], vf);
+            weight_row(i, gate, vw);
+            if (!kOneGate && p.gate) Elem<KIND>::unpack(gate.w[i], vg);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float tf = t[i][j] * (vf[j] * rf);
-            dot[0] += t[i][j] * vw[j] * vf[j];
-            if constexpr (kOneGate) {
-              acc_post[i][j] += tf;
-            } else {
-              acc_post[i][j] += p.gate ? vg[j] * tf : tf;
-              acc_gate[i][j] += tf;
+            for (int j = 0; j < V; ++j) {
+              const float tf = t[i][j] * (vf[j] * rf);
+              dot[0] += t[i][j] * vw[j] * vf[j];
+              if constexpr (kOneGate) {
+                acc_post[i][j] += tf;
+              } else {
+                acc_post[i][j] += p.gate ? vg[j] * tf : tf;
+                acc_gate[i][j] += tf;
+              }
             }
           }
         }
-      }
       }
       // the next row is requested here, ahead of this row's stores and second round of sums; rows of
       // several pieces per lane have no registers for two rows and request theirs when they are done
