@@ -332,9 +332,12 @@ def _rows(t, shape, dtype, index, what):
 
 def _given_stream(stream, index):
     """The caller's stream as the current one, for a call's results and scratch as well: memory
-    from another stream's pool may still be in use by work that is under way there."""
+    from another stream's pool may still be in use by work that is under way there.  0 is the
+    default stream's handle (ExternalStream would take it for "any stream of the pool", which
+    waits for nothing that the caller has issued)."""
     import torch
-    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=index))
+    given = torch.cuda.ExternalStream(stream, device=index) if stream else torch.cuda.default_stream(index)
+    return torch.cuda.stream(given)
 
 
 def _launch_on(index, symbol, block_dim, tiling, workspace, *tensors):

@@ -363,3 +363,30 @@ def test_a_given_stream(H):
     got = backward(H, v, y, 1, stream=s.cuda_stream)
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_default_stream_given_by_its_handle(H, monkeypatch):
+    """stream=0 is the default stream, as for every other launcher, from whatever stream the call is made."""
+    assert torch.cuda.default_stream().cuda_stream == 0
+    v = inputs(40, 96, 1, "bf16", 18)
+    y, h = forward(H, v, 1)
+    grads = backward(H, v, y, 1)
+    q = H.mxfp4_quantize(v["x"])
+    out = H.mxfp4_matmul_add_leakyrelu(*q, *q)
+    torch.cuda.synchronize()
+    used, launch = [], H._launch_on
+
+    def recorded(index, *rest):
+        used.append(torch.cuda.current_stream(index).cuda_stream)
+        return launch(index, *rest)
+
+    monkeypatch.setattr(H, "_launch_on", recorded)
+    for place in (torch.cuda.default_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(place):
+            got = (*forward(H, v, 1, stream=0), *backward(H, v, y, 1, stream=0), *H.mxfp4_quantize(v["x"], stream=0),
+                   H.mxfp4_matmul_add_leakyrelu(*q, *q, stream=0))
+            assert torch.cuda.current_stream() == place
+        torch.cuda.synchronize()
+        for a, b in zip(got, (y, h, *grads, *q, out)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert used == [0] * 8
