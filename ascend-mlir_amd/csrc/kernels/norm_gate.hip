@@ -15,6 +15,8 @@
 //
 // bf16 8192 x 4096, a gate per 2048 rows: forward 46 us (5.8 TB/s), backward 87 and 8 for the join of the
 // column sums (4.6 TB/s; some 350 vector instructions a row and wavefront keep the vector units half busy).
+#include <utility>
+
 #include "kernels.h"
 #include "mxfp4.h"
 
@@ -598,6 +600,20 @@ LaunchStatus backward(const NormGateGradArgs &p, uint32_t block_dim, hipStream_t
   }
 }
 
+// Whether two results of m rows of n numbers share one: rows of one stride by what the starts are apart,
+// modulo the stride; rows of different strides as soon as the stretches of memory that they span do.
+bool results_overlap(const void *a, int64_t ld_a, const void *b, int64_t ld_b, int64_t m, int64_t n, int64_t size) {
+  if (reinterpret_cast<uintptr_t>(a) > reinterpret_cast<uintptr_t>(b)) {
+    std::swap(a, b);
+    std::swap(ld_a, ld_b);
+  }
+  const uint64_t apart = (reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) / (uint64_t)size;
+  if (apart >= (uint64_t)((m - 1) * ld_a + n)) return false;
+  if (ld_a != ld_b) return true;
+  const int64_t rows = (int64_t)apart / ld_a, within = (int64_t)apart % ld_a;   // b starts in row `rows` of a, or behind it
+  return within < n || (within > ld_a - n && rows + 1 < m);
+}
+
 }  // namespace
 
 LaunchStatus launch_norm_gate_residual(const NormGateArgs &args, int elem_kind, uint32_t block_dim, hipStream_t stream) {
@@ -620,6 +636,8 @@ LaunchStatus launch_norm_gate_residual(const NormGateArgs &args, int elem_kind, 
   const uintptr_t elem = elem_kind == kElemF32 ? 4 : 2;
   for (const void *q : {p.x, p.f, p.gate, p.post_weight, p.pre_weight, (const void *)p.y, (const void *)p.h})
     if (reinterpret_cast<uintptr_t>(q) % elem) return invalid("norm_gate_residual: tensor off its element's alignment");
+  if (p.y && p.h && results_overlap(p.y, p.ld_y, p.h, p.ld_h, p.m, p.n, elem))
+    return invalid("norm_gate_residual: y and h are two results and must not overlap");
   p.inv_n = (float)(1.0 / (double)p.n);
   if (p.rows_per_gate > p.m) p.rows_per_gate = p.m;
   switch (elem_kind) {
@@ -666,6 +684,8 @@ LaunchStatus launch_norm_gate_residual_backward(const NormGateGradArgs &args, in
     if (reinterpret_cast<uintptr_t>(q) % elem)
       return invalid("norm_gate_residual_backward: tensor off its element's alignment");
   if (reinterpret_cast<uintptr_t>(p.partial) % 4) return invalid("norm_gate_residual_backward: workspace off a 4-byte boundary");
+  if (p.f && results_overlap(p.dx, p.ld_dx, p.df, p.ld_df, p.m, p.n, elem))
+    return invalid("norm_gate_residual_backward: dx and df are two results and must not overlap");
   p.inv_n = (float)(1.0 / (double)p.n);
   if (p.rows_per_gate > p.m) p.rows_per_gate = p.m;
   switch (elem_kind) {

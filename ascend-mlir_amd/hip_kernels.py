@@ -490,7 +490,7 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
     x, f [M, N] (rows may have a stride), weights [N], gate [G, N] or [N]: row i takes gate
     row i // rows_per_gate (None: one gate row for all rows, or one each).  Without f, y is x
     (the norm ahead of the first block); without pre_weight there is no h.  Returns (y, h).
-    y=x and h=f work in place."""
+    y=x and h=f work in place; y and h must not overlap."""
     index = _device_of(x, "x")
     if stream is not None:
         with _given_stream(stream, index):

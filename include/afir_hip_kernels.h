@@ -202,7 +202,8 @@ size_t afir_hip_mxfp4_matmul_workspace_bytes(const void *tiling);
  * gate [ceil(M/rows_per_gate), N]: row i takes gate row i / rows_per_gate.
  * f NULL (then also post_weight, gate and y): y is x itself, the norm ahead of
  * the first block.  pre_weight NULL (then also h): no second norm.  gate NULL:
- * 1.  y may be x and h may be f.  N at most 16384.
+ * 1.  y may be x and h may be f; y and h must not overlap (in one stretch of
+ * memory, side by side, their rows need one stride).  N at most 16384.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;
  *              int64 ld_x, ld_f, ld_gate, ld_y, ld_h;
  *              int64 residual_scale_f32_bits; int64 eps_f32_bits; int64 elem_type } */
@@ -214,7 +215,8 @@ uint32_t afir_hip_launch_norm_gate_residual(uint32_t block_dim, void *stream, vo
  * wrote: dx, df [M,N], dpost_weight, dpre_weight [N], dgate like gate (densely
  * packed).  dy NULL: zero.  dh NULL (then also y, pre_weight, dpre_weight): the
  * call had no h.  f NULL (then also post_weight, gate and their gradients and
- * df): it had no f.  dx may be dy and df may be f.  workspace: a device buffer
+ * df): it had no f.  dx may be dy and df may be f; dx and df must not overlap,
+ * as y and h above.  workspace: a device buffer
  * of afir_hip_norm_gate_residual_backward_workspace_bytes(tiling) bytes, one
  * for each of the launches that may overlap.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;

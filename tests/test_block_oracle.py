@@ -204,6 +204,22 @@ def test_norm_backward_refuses(H, args, fields, word):
     assert "null tiling" in refusal(H, GRAD, a.values(), f.values(), bad_tiling=True)
 
 
+# y and h, dx and df: (bytes from the first result to the second, their row strides), m = 4, n = 64, two bytes a number
+@pytest.mark.parametrize("apart,ld_first,ld_second", [
+    (0, 64, 64), (2, 64, 64), (126, 64, 64), (3 * 128, 64, 64), (4 * 128 - 2, 64, 64),   # dense rows
+    (0, 200, 200), (126, 200, 200), (200 * 2 - 126, 200, 200), (2 * 400 + 126, 200, 200), (3 * 400 + 126, 200, 200),
+    (2 * 400 + 400 - 126, 200, 200), (0, 64, 200), (128, 200, 64), (3 * 400 + 126, 200, 64)])
+def test_norms_refuse_two_results_that_overlap(H, apart, ld_first, ld_second):
+    for first, second in (("y", "h"), ("h", "y")):
+        a = dict(ALL, **{first: FAKE, second: FAKE + apart})
+        f = dict(FIELDS, **{"ld_" + first: ld_first, "ld_" + second: ld_second})
+        assert "must not overlap" in refusal(H, NORM, (*a.values(), 0), f.values())
+    for first, second in (("dx", "df"), ("df", "dx")):
+        a = dict(GALL, **{first: FAKE, second: FAKE + apart})
+        f = dict(GFIELDS, **{"ld_" + first: ld_first, "ld_" + second: ld_second})
+        assert "must not overlap" in refusal(H, GRAD, a.values(), f.values())
+
+
 def test_empty_calls_launch_nothing(H):
     L = H.load()
     null = [ctypes.c_void_p(0)]

@@ -236,6 +236,26 @@ def test_two_results_in_one_tensor_are_refused(H):
         H.norm_gate_residual(v["x"], v["f"], v["post_weight"], v["gate"], v["pre_weight"], y=t, h=t)
 
 
+def test_two_results_in_one_buffer(H):
+    """Views that share numbers are refused, whatever objects they are; views side by side are not."""
+    m, n = 5, 96
+    v = inputs(m, n, 1, "bf16", 21)
+    y, h = forward(H, v, 1)
+    t = torch.full((m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    wide = torch.full((m + 1, 3 * n), 7.0, dtype=torch.bfloat16, device="cuda")
+    for a, b in ((t, t.view(m, n)), (t.view(m, n), t), (wide[:m, :n], wide[:m, n - 1:2 * n - 1]),
+                 (wide[1:, :n], wide.as_strided((m, n), (3 * n, 1), 2 * n + 1)),
+                 (wide[:m, :n], wide[1:, :n])):
+        with pytest.raises(H.AfirHipError, match="must not overlap"):
+            forward(H, v, 1, y=a, h=b)
+    assert (t == 7).all() and (wide == 7).all()
+    stacked = torch.empty((2 * m, n), dtype=torch.bfloat16, device="cuda")
+    for a, b in ((wide[:m, :n], wide[:m, n:2 * n]), (wide[1:, n:2 * n], wide[1:, :n]), (wide[:m, 2 * n:], wide[1:, :n]),
+                 (wide[1:, :n], wide[:m, n:2 * n]), (stacked[:m], stacked[m:]), (stacked[m:], stacked[:m])):
+        forward(H, v, 1, y=a, h=b)
+        assert torch.equal(a, y) and torch.equal(b, h)
+
+
 def test_refusals(H):
     v = inputs(8, 64, 2, "bf16", 16)
     x, f, w, gate = v["x"], v["f"], v["post_weight"], v["gate"]
