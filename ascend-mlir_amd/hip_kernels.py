@@ -476,7 +476,8 @@ def _gate_rows(gate, m, n, rows_per_gate, dtype, index):
     g = gate.shape[0]
     if rows_per_gate is None:
         rows_per_gate = max(m, 1) if g == 1 else 1
-    if rows_per_gate < 1 or -(-m // rows_per_gate) != g:
+    # (a batch of no rows needs no gate row, and may come with the one learned row of every batch)
+    if rows_per_gate < 1 or (-(-m // rows_per_gate) != g and (m, g) != (0, 1)):
         raise AfirHipError(f"gate: {g} rows of {rows_per_gate} do not cover {m} rows")
     return rows_per_gate, _rows(gate, (g, n), dtype, index, "gate")
 

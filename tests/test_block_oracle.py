@@ -240,3 +240,20 @@ def test_host_tensors_are_refused(H):
         H.norm_gate_residual_backward(x, x, x, pre_weight=x[0])
     with pytest.raises(H.AfirHipError, match="device tensor"):
         H.mxfp4_matmul_add_leakyrelu(x, x, x, x)
+
+
+@pytest.mark.parametrize("gate,rows_per_gate", [((24,), None), ((1, 24), None), ((1, 24), 7), ((0, 24), None), ((0, 24), 3),
+                                                (None, None)])
+def test_a_batch_of_no_rows_goes_with_a_learned_gate(H, monkeypatch, gate, rows_per_gate):
+    """The host side alone: what would be launched is recorded."""
+    import torch
+    launched = []
+    monkeypatch.setattr(H, "_device_of", lambda t, what: -1)   # host tensors pass for those of one device
+    monkeypatch.setattr(H, "_launch_on", lambda index, symbol, block_dim, tiling, *rest: launched.append(tiling))
+    x, w = torch.zeros(0, 24), torch.ones(24)
+    gate = None if gate is None else torch.ones(gate)
+    y, h = H.norm_gate_residual(x, x.clone(), w, gate, w, rows_per_gate=rows_per_gate)
+    assert y.shape == h.shape == (0, 24) and len(launched) == 1
+    for bad, per in ((torch.ones(2, 24), None), (torch.ones(2, 24), 1), (torch.ones(1, 24), 0)):
+        with pytest.raises(H.AfirHipError, match="do not cover"):
+            H.norm_gate_residual(x, x.clone(), w, bad, w, rows_per_gate=per)
