@@ -117,9 +117,12 @@ template <int NT, int KIND>
 LaunchStatus rows_launch(const MxOperands &p, uint32_t block_dim, hipStream_t stream) {
   const int tiles_n = (p.n + 16 * NT - 1) / (16 * NT), chunks_m = (p.m + 15) / 16;
   const int64_t blocks = (int64_t)((tiles_n + kNumXCD - 1) / kNumXCD) * kNumXCD * chunks_m;
-  if (blocks > 0x7fffffff) return invalid("mxfp4_matmul: too many output tiles");
-  AFIR_LAUNCH("mxfp4_matmul_rows", (mxfp4_matmul_rows<NT, KIND>), dim3(block_dim ? block_dim : (unsigned)blocks),
-              dim3(kRowsWaves * 64), 0, stream, p, tiles_n, chunks_m, (int)blocks);
+  // (a launch holds less than 2^32 threads, 2^23 workgroups of these; beyond the bound they take several places)
+  constexpr int64_t kMost = (int64_t)1 << 20;
+  if (blocks > 0x7fffffff - kMost) return invalid("mxfp4_matmul: too many output tiles");
+  const int64_t grid = block_dim ? block_dim : blocks < kMost ? blocks : kMost;
+  AFIR_LAUNCH("mxfp4_matmul_rows", (mxfp4_matmul_rows<NT, KIND>), dim3((unsigned)grid), dim3(kRowsWaves * 64), 0, stream, p,
+              tiles_n, chunks_m, (int)blocks);
   return after_launch();
 }
 

@@ -341,3 +341,30 @@ def test_matmul_refuses(H):
                            ((torch.zeros(4 * 32 + 1, **u8)[1:].view(4, 32), sa, b, sb), {}, "16-byte")):
         with pytest.raises(H.AfirHipError, match=word):
             H.mxfp4_matmul_add_leakyrelu(*args, **kw)
+
+
+def random_operand(rows, kb, gen):
+    """Codes and scales made on the GPU: any code, scales of 2^-3 to 2^3."""
+    codes = torch.randint(0, 256, (rows, kb * 16), dtype=torch.uint8, device="cuda", generator=gen)
+    return codes, torch.randint(124, 131, (rows, kb), dtype=torch.uint8, device="cuda", generator=gen)
+
+
+def decoded(operand, rows):
+    return O.decode(operand[0][rows].cpu().numpy(), operand[1][rows].cpu().numpy())
+
+
+def test_matmul_of_more_columns_than_a_launch_has_threads(H):
+    # 2^28 columns and some: 2^23 tiles of 32 columns and 512 threads each
+    n, gen = (1 << 28) + 77, torch.Generator(device="cuda").manual_seed(6)
+    a, b = random_operand(1, 1, gen), random_operand(n, 1, gen)
+    e8 = torch.float8_e8m0fnu
+    out = torch.full((n + 64,), 77.0, dtype=torch.bfloat16, device="cuda")
+    got = H.mxfp4_matmul_add_leakyrelu(a[0], a[1].view(e8), b[0], b[1].view(e8), alpha=0.25, out=out[:n].view(1, n))
+    assert H.last_launch()["kernel"] == "mxfp4_matmul_rows"
+    torch.cuda.synchronize()
+    assert (out[n:] == 77).all()
+    # the first and the last columns, both sides of each bound on the way, and some from everywhere
+    some = torch.cat([torch.arange(at - 70, at + 70) for at in (70, 1 << 25, 1 << 26, 1 << 27, 1 << 28, n - 70)] +
+                     [torch.randint(0, n, (20000,))]).cuda()
+    want, size = O.matmul(decoded(a, slice(None)), decoded(b, some), None, 0.25)
+    B.close(got[:, some], want, size, "bf16", 11)
