@@ -368,3 +368,84 @@ def test_matmul_of_more_columns_than_a_launch_has_threads(H):
                      [torch.randint(0, n, (20000,))]).cuda()
     want, size = O.matmul(decoded(a, slice(None)), decoded(b, some), None, 0.25)
     B.close(got[:, some], want, size, "bf16", 11)
+
+
+@pytest.mark.parametrize("kind", B.TYPES)
+@pytest.mark.parametrize("m,n,k,blocks", [
+    # 32 columns a workgroup (n above 16 per compute unit), the last ones partly past the end; more steps of 512 numbers
+    # than the eight wavefronts take in one go, the last step whole or not
+    (1, 4097, 4096, 0), (7, 4129, 4128, 0), (16, 8200, 608, 0), (16, 4128, 8192, 0), (1, 5003, 8192 + 416, 0),
+    (7, 4100, 8192 + 512, 37), (16, 4129, 32, 5), (1, 8224, 65, 0),
+    # 16 columns a workgroup, as deep
+    (1, 520, 8192 + 416, 0), (16, 72, 4096 + 512, 0), (7, 4096, 4128, 3), (3, 17, 3 * 4096 + 32, 0)])
+def test_matmul_of_few_rows(H, kind, m, n, k, blocks):
+    check_matmul(H, m, n, k, kind, block_dim=blocks)
+    last, tiles = H.last_launch(), -(-n // (32 if n > 4096 else 16))
+    assert last["kernel"] == "mxfp4_matmul_rows" and last["workgroups"] == (blocks or -(-tiles // 8) * 8)
+    check_matmul(H, m, n, k, kind, bias=False, alpha=1.0, seed=1, block_dim=blocks)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4129, 8192 + 416), (16, 4100, 4128), (5, 300, 8192 + 96)])
+def test_matmul_of_few_rows_keeps_nan_and_scales_at_their_ends(H, m, n, k):
+    rng = np.random.default_rng(7)
+    (ac, asc), (bc, bsc) = operand(rng, m, k), operand(rng, n, k)
+    asc[:], bsc[:] = 0, 254
+    asc[:, ::2], bsc[:, ::2] = 250, 4
+    if m > 1:
+        asc[m - 1, -1] = 255
+    bsc[n - 1, -1] = bsc[7, -9] = bsc[40, 128] = 255
+    want, size = O.matmul(O.decode(ac, asc), O.decode(bc, bsc), None, 1.0)
+    dev = [torch.from_numpy(t).cuda() for t in (ac, asc, bc, bsc)]
+    got = H.mxfp4_matmul_add_leakyrelu(dev[0], dev[1].view(torch.float8_e8m0fnu), dev[2], dev[3].view(torch.float8_e8m0fnu),
+                                       alpha=1.0, out_dtype=torch.float32)
+    lost = np.zeros((m, n), dtype=bool)
+    lost[:, [7, 40, n - 1]] = True
+    if m > 1:
+        lost[m - 1] = True
+    assert np.array_equal(np.isnan(got.cpu().numpy()), lost)
+    if not lost.all():
+        B.close(got[torch.from_numpy(~lost).cuda()], want[~lost], size[~lost], "f32", -(-k // 32) + 10)
+
+
+@pytest.mark.parametrize("m,n,k,threads", [(4100, 4200, 1056, 512), (2100, 2100, 608, 256), (2200, 2050, 1280, 256)])
+def test_matmul_on_tiles_keeps_nan_and_scales_at_their_ends(H, m, n, k, threads):
+    """Both tiles of the kernel with persistent workgroups: 256 x 256 with eight wavefronts, 128 x 128 with four."""
+    test_matmul_of_many_rows_keeps_nan_and_scales_at_their_ends(H, m, n, k)
+    last = H.last_launch()
+    assert last["kernel"] == "mxfp4_matmul_tiles" and last["threads"] == threads
+
+
+# ---- more than 2^31 numbers ----
+
+@pytest.mark.parametrize("axis", [1, 0])
+def test_quantize_beyond_32_bit_offsets(H, axis):
+    rows, k = 133000, 16416
+    x = torch.randn((rows, k) if axis else (k, rows), device="cuda", dtype=torch.bfloat16)
+    codes, scales, values = H.mxfp4_quantize(x, axis=axis, return_values=True)
+    for part in (slice(0, 40), slice(130780, 130860), slice(rows - 40, rows)):   # 2^31 numbers are 130816 rows and some
+        piece = x[part] if axis else x[:, part]
+        want = O.quantize(B.numbers(piece) if axis else B.numbers(piece).T)
+        assert np.array_equal(codes[part].cpu().numpy(), want[0])
+        assert np.array_equal(scales[part].view(torch.uint8).cpu().numpy(), want[1])
+        assert np.array_equal(B.numbers(values[part] if axis else values[:, part]), want[2] if axis else want[2].T)
+
+
+def test_quantize_more_rows_than_one_launch_takes(H):
+    rows = (1 << 29) + 70     # of one number: a launch indexes 2^31 groups of eight, four to a block
+    x = torch.randint(-8, 9, (rows, 1), device="cuda", dtype=torch.int8).to(torch.float16)
+    codes, scales = H.mxfp4_quantize(x)
+    some = torch.cat([torch.arange(200), torch.arange((1 << 29) - 100, rows), torch.randint(0, rows, (5000,))]).cuda()
+    want = O.quantize(B.numbers(x[some]))
+    assert np.array_equal(codes[some].cpu().numpy(), want[0])
+    assert np.array_equal(scales[some].view(torch.uint8).cpu().numpy(), want[1])
+
+
+def test_matmul_beyond_32_bit_offsets(H):
+    m, n, gen = 66000, 33000, torch.Generator(device="cuda").manual_seed(8)
+    a, b = random_operand(m, 9, gen), random_operand(n, 9, gen)
+    e8 = torch.float8_e8m0fnu
+    got = H.mxfp4_matmul_add_leakyrelu(a[0], a[1].view(e8), b[0], b[1].view(e8), alpha=0.5)
+    assert H.last_launch()["kernel"] == "mxfp4_matmul_tiles"
+    for part in (slice(0, 20), slice(65060, 65090), slice(m - 20, m)):   # 2^31 numbers are 65075 rows and some
+        want, size = O.matmul(decoded(a, part), decoded(b, slice(None)), None, 0.5)
+        B.close(got[part], want, size, "bf16", 19)
