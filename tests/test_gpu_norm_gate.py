@@ -410,3 +410,116 @@ def test_the_default_stream_given_by_its_handle(H, monkeypatch):
         for a, b in zip(got, (y, h, *grads, *q, out)):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     assert used == [0] * 8
+
+
+def signs(rng, shape):
+    return rng.integers(0, 2, shape) * 2.0 - 1
+
+
+def terms(rng, m, n):
+    """m rows of +-1 whose column sums stay small: half of the rows undo the other half, but for sixty at the end."""
+    c = signs(rng, (m, n))
+    half = (m - 60) // 2
+    if half > 0:
+        c[half:2 * half] = -c[rng.permutation(half)]
+    return c
+
+
+@pytest.mark.parametrize("kind,m,n,rows_per_gate", [
+    ("bf16", 8192, 64, 3), ("f32", 8200, 64, 10), ("f16", 8191, 256, 20), ("bf16", 4097, 512, 2), ("f32", 5000, 256, 1),
+    ("f16", 4100, 1024, 9), ("bf16", 6001, 1024, 700), ("f32", 3000, 1024, 11), ("f16", 2600, 2048, 3), ("bf16", 2100, 2048, 7),
+    ("f32", 2049, 512, 2049), ("bf16", 8192, 64, 0), ("bf16", 1500, 4096, 0), ("f16", 1100, 8192, 300), ("bf16", 700, 16384, 0),
+    ("f32", 600, 8192, 5), ("f32", 520, 16384, 100), ("bf16", 513, 4096, 17), ("f16", 40, 2048, 0), ("f32", 3, 64, 2)])
+def test_column_sums_miss_no_row_and_take_none_twice(H, kind, m, n, rows_per_gate):
+    """Rows of +-1 have the norm 1, so with weights and gates of 1 every term of a column sum is +-1: the sums are whole
+    numbers that each of the types holds, compared without a tolerance."""
+    rng = np.random.default_rng(m + n)
+    per = rows_per_gate or m
+    t = lambda a: B.tensor(a, kind, "cuda")
+    f, y, c, d = signs(rng, (m, n)), signs(rng, (m, n)), terms(rng, m, n), terms(rng, m, n)
+    one, starts = t(np.ones(n)), np.arange(0, m, per)
+    gate = t(np.ones((len(starts), n))) if rows_per_gate else None
+    sums, dgate = c.sum(axis=0), np.add.reduceat(c, starts, axis=0)
+    assert np.abs(sums).max() <= 256 and np.abs(dgate).max() <= 256
+    got = H.norm_gate_residual_backward(t(c * f), None, t(y), t(f), one, gate, eps=0.0, rows_per_gate=rows_per_gate or None)
+    assert np.array_equal(B.numbers(got[2]), sums)
+    if gate is not None:
+        assert np.array_equal(B.numbers(got[3]), dgate)
+    got = H.norm_gate_residual_backward(t(c * f), t(d * y), t(y), t(f), one, gate, one, eps=0.0,
+                                        rows_per_gate=rows_per_gate or None)
+    assert np.array_equal(B.numbers(got[4]), d.sum(axis=0))
+    got = H.norm_gate_residual_backward(None, t(d * y), t(y), pre_weight=one, eps=0.0)
+    assert np.array_equal(B.numbers(got[4]), d.sum(axis=0))
+
+
+GRAD = "afir_hip_launch_norm_gate_residual_backward"
+
+
+def launch_backward(H, v, y, kind, rows_per_gate, dx, df, dy, f):
+    """The C launcher: results in given places, whose rows have the strides that they have."""
+    m, n = y.shape
+    gate = v["gate"]
+    dpost, dpre = torch.empty_like(v["post_weight"]), torch.empty_like(v["pre_weight"])
+    dgate = None if gate is None else torch.empty_like(gate)
+    tiling = H.pack_tiling(m, n, rows_per_gate or m, dy.stride(0), n, n, f.stride(0), n, dx.stride(0), df.stride(0),
+                           H.f32_bits(SCALE), H.f32_bits(EPS), list(B.TYPES).index(kind))
+    size = H.load().afir_hip_norm_gate_residual_backward_workspace_bytes(tiling)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    ptrs = [0 if t is None else t.data_ptr() for t in (dy, v["dh"], y, f, v["post_weight"], gate, v["pre_weight"], dx, df,
+                                                       dpost, dgate, dpre, workspace)]
+    assert H.launch_raw(GRAD, 0, None, ptrs, tiling) == 0
+    torch.cuda.synchronize()
+    return dx, df, dpost, dgate, dpre
+
+
+@pytest.mark.parametrize("kind,m,n,rows_per_gate", [
+    # rows of 1 to 16 wavefronts and of 1, 2 and 4 pieces per lane; gates within a stretch, over several, and none
+    ("bf16", 900, 200, 1), ("f32", 1500, 200, 700), ("f16", 2500, 600, 7), ("bf16", 1200, 2000, 0), ("f32", 700, 2048, 3),
+    ("f16", 600, 5000, 600), ("bf16", 1030, 9000, 40), ("f32", 530, 16000, 1), ("f16", 50, 16384, 7), ("bf16", 1, 300, 1)])
+def test_gradients_in_place_and_with_strides(H, kind, m, n, rows_per_gate):
+    v = inputs(m, n, rows_per_gate, kind, 22)
+    y, _ = forward(H, v, rows_per_gate)
+    want = backward(H, v, y, rows_per_gate)
+
+    def same(got):
+        for a, b in zip(got, want):
+            assert (a is None and b is None) or torch.equal(a, b)
+
+    # dx in dy's place, df in f's
+    dy, f = v["dy"].clone(), v["f"].clone()
+    same(launch_backward(H, v, y, kind, rows_per_gate, dy, f, dy, f))
+
+    def wide(t, left, right):
+        big = torch.full((m, left + n + right), 77.0, dtype=t.dtype, device="cuda")
+        big[:, left:left + n] = t
+        return big, big[:, left:left + n]
+
+    def untouched(big, left):
+        return (big[:, :left] == 77).all() and (big[:, left + n:] == 77).all()
+
+    # rows with strides of their own, off every boundary but an element's
+    (big_dx, dx), (big_df, df) = wide(torch.zeros_like(y), 3, 6), wide(torch.zeros_like(y), 1, 4)
+    same(launch_backward(H, v, y, kind, rows_per_gate, dx, df, v["dy"], v["f"]))
+    assert untouched(big_dx, 3) and untouched(big_df, 1)
+    # ... and in place with them
+    (big_dy, dy), (big_f, f) = wide(v["dy"], 3, 6), wide(v["f"], 1, 4)
+    same(launch_backward(H, v, y, kind, rows_per_gate, dy, f, dy, f))
+    assert untouched(big_dy, 3) and untouched(big_f, 1)
+
+
+def test_beyond_32_bit_offsets(H):
+    m, n, per, kind = 133000, 16384, 1000, "bf16"      # 2^31 numbers are 131072 rows
+    r = lambda rows, spread: torch.randn(rows, n, device="cuda", dtype=torch.bfloat16) * spread
+    v = dict(x=r(m, 3), f=r(m, 2), dy=r(m, 0.5), dh=r(m, 0.5), post_weight=r(1, 1)[0], pre_weight=r(1, 1)[0],
+             gate=torch.sigmoid(r(m // per, 1)))
+    got = forward(H, v, per)
+    grads = backward(H, v, got[0], per)
+    for first, last in ((0, 20), (131000, 131100), (132980, 133000)):
+        part = {k: t if t.dim() == 1 else t[first:last] for k, t in v.items()}
+        part["gate"] = v["gate"][first // per:first // per + 1]
+        check_forward(part, [t[first:last] for t in got], kind, per)
+        ref, y = reference(part), B.numbers(got[0][first:last])
+        want, size = O.norm_grad(ref["dy"], ref["dh"], y, ref["f"], ref["post_weight"], ref["gate"], ref["pre_weight"], SCALE,
+                                 EPS, per)
+        for name, g in zip(("dx", "df"), grads):
+            B.close(g[first:last], want[name], size[name], kind, 3 * B.row_sum_steps(n) + 24)
