@@ -182,7 +182,7 @@ LaunchStatus direct_launch(const MxOperands &p, uint32_t block_dim, hipStream_t 
   return after_launch();
 }
 
-// A tile per workgroup up to 64 rows (9.2 us against 15.8 on the kernel of few rows at 48 x 8200 x 4096), and while
+// A tile per workgroup up to 64 rows (8.7 us against 15.8 on the kernel of few rows at 48 x 8200 x 4096), and while
 // each compute unit gets at most one of 128 x 128 (512 x 8192 x 8192: 27 us, 28 on tiles in turn); beyond that
 // tiles in turn (1024 x 8192 x 8192: 45 us against 55).
 bool one_tile_each(const MxOperands &p) {

@@ -15,8 +15,8 @@
 //
 // How deep the ring is (3, 4 or 8 slots) measured the same.  What a slice costs is its issue, LDS and
 // barrier time: requesting the next lines between the products took 512 x 8192 x 8192 from 28.3 to 26.1 us;
-// the smaller tiles hide it in the other workgroups of their compute unit.  Measured: 48 x 8200 x 4096 9.2 us,
-// 128 x 8192 x 8192 14.6, 256 x 8192 x 8192 19.8, 1003 x 2056 x 1376 10.5, 1024 x 4096 x 4096 16.
+// the smaller tiles hide it in the other workgroups of their compute unit.  Measured: 48 x 8200 x 4096 8.7 us,
+// 128 x 8192 x 8192 14.6, 256 x 8192 x 8192 19.6, 1003 x 2056 x 1376 10.1 (11.1 into float32), 1024 x 4096 x 4096 17.
 #include "mxfp4_mfma.h"
 
 namespace afir {

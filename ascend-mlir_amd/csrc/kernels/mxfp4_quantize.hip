@@ -43,7 +43,8 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 // 16-bit types, a scale from two steps across the quad.  The (row, quad) pairs are dealt out flat,
 // so rows of any length fill the wavefronts; a lane asks for kUnroll groups before it uses the
 // first.  `groups` is a row's lanes, four to a block; numbers past the row's end count as zeros.
-// bf16 8192 x 8192 with values: 48.5 us (6.3 TB/s), 51.4 with values stored by way of the L2.
+// bf16 8192 x 8192 with values: 48.5 us (6.3 TB/s), 51.4 with values stored by way of the L2; without values 29
+// (5.9 TB/s).  float32, whose lanes take two pieces 32 bytes apart: 107 (5.4 TB/s), without values 54.
 template <int KIND, bool VALUES>
 __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows(const void *__restrict__ x, int64_t ld,
                                                                 uint32_t *__restrict__ codes,
@@ -139,8 +140,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows(const void *__re
 // The eight blocks of a column meet in LDS and leave as whole 128-byte lines of its code row.  Rows that
 // are no whole number of lines share lines between neighbouring tiles, which therefore belong to one XCD,
 // whose L2 puts them together: float32 [8192, 4099] with values 54 us against 72 with neighbours on
-// different XCDs (and 71 with stores that bypass the L2); 62 us (4.6 TB/s) where the output is not in the
-// last-level cache from the call before.
+// different XCDs (and 71 with stores that bypass the L2); 63 us (4.5 TB/s) where the output is not in the
+// last-level cache from the call before.  bf16 [8192, 8192]: 66 us (4.6 TB/s), without values 43.
 constexpr int kColWaves = 8;
 template <int KIND, bool VALUES>
 __global__ __launch_bounds__(kColWaves * 64) void mxfp4_quantize_cols(const void *__restrict__ x, int64_t ld,

@@ -262,7 +262,8 @@ def matmul_add_leakyrelu(a, b, bias, alpha=0.01, out=None, block_dim=0, stream=N
 # Unlike the families above these take tensors of any of the three float types and rows
 # with a stride, launch on the device of their tensors, and check every tensor against the
 # others before they launch.  They are called once per layer and token, so the checks are
-# one expression per tensor; only a tensor that fails it is looked at closely.
+# one expression per tensor; only a tensor that fails it is looked at closely.  Autograd does
+# not see them: results carry no graph, also where an input requires a gradient.
 
 _ELEM_TYPES = {}
 _entries = {}
@@ -491,7 +492,8 @@ def norm_gate_residual(x, f=None, post_weight=None, gate=None, pre_weight=None, 
     x, f [M, N] (rows may have a stride), weights [N], gate [G, N] or [N]: row i takes gate
     row i // rows_per_gate (None: one gate row for all rows, or one each).  Without f, y is x
     (the norm ahead of the first block); without pre_weight there is no h.  Returns (y, h).
-    y=x and h=f work in place; y and h must not overlap."""
+    y=x and h=f work in place; y and h must not overlap.  The results carry no autograd graph:
+    norm_gate_residual_backward gives the gradients."""
     index = _device_of(x, "x")
     if stream is not None:
         with _given_stream(stream, index):
@@ -534,7 +536,8 @@ def norm_gate_residual_backward(dy, dh, y, f=None, post_weight=None, gate=None, 
                                 eps=1e-6, rows_per_gate=None, block_dim=0, stream=None):
     """The gradients (dx, df, dpost_weight, dgate, dpre_weight) of norm_gate_residual from
     those of its results and the y it returned; None where it had no such input.  dy None:
-    zero.  dh, pre_weight None: the call had no h (y is not read then)."""
+    zero.  dh, pre_weight None: the call had no h (y is not read then).  An empty y is refused:
+    there are no rows to sum the weights' gradients over."""
     index = _device_of(y, "y")
     if stream is not None:
         with _given_stream(stream, index):

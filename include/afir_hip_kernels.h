@@ -183,11 +183,12 @@ uint32_t afir_hip_launch_mxfp4_quantize(uint32_t block_dim, void *stream, void *
  * K as quantised above, bias [N] (NULL: none) and out [M,N] of elem_type.  The
  * products of codes are exact and are added in float32 on the matrix cores
  * (v_mfma_scale_f32_16x16x128_f8f6f4).  The scale byte 255 makes every number
- * that its block enters a NaN.  workspace: NULL, or a device buffer on a
- * 16-byte boundary of afir_hip_mxfp4_matmul_workspace_bytes(tiling) bytes,
- * which lets large products run on a faster kernel (0: they run on it without);
- * a launch leaves nothing in
- * it that a later one reads, but launches that may overlap need one each.
+ * that its block enters a NaN.  The maximum is fmaxf's: where v*alpha is a NaN
+ * and v is not (alpha 0, v infinite), out is v.  workspace: NULL, or a device
+ * buffer on a 16-byte boundary of afir_hip_mxfp4_matmul_workspace_bytes(tiling)
+ * bytes, which lets large products run on a faster kernel (0: the product runs
+ * on one that takes no workspace).  A launch leaves nothing in it that a later
+ * one reads, but launches that may overlap need one each.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (K); int64 dim_arg2_0 (N);
  *              int64 alpha_f32_bits; int64 elem_type }                         */
 uint32_t afir_hip_launch_mxfp4_matmul_add_leakyrelu(uint32_t block_dim, void *stream, void *a,
@@ -203,7 +204,9 @@ size_t afir_hip_mxfp4_matmul_workspace_bytes(const void *tiling);
  * f NULL (then also post_weight, gate and y): y is x itself, the norm ahead of
  * the first block.  pre_weight NULL (then also h): no second norm.  gate NULL:
  * 1.  y may be x and h may be f; y and h must not overlap (in one stretch of
- * memory, side by side, their rows need one stride).  N at most 16384.
+ * memory, side by side, their rows need one stride).  N at most 16384.  Row sums
+ * are float32: a row whose sum of squares passes its range (numbers near 1e19)
+ * is out of the norms' range, here and in the gradients.  M = 0 launches nothing.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;
  *              int64 ld_x, ld_f, ld_gate, ld_y, ld_h;
  *              int64 residual_scale_f32_bits; int64 eps_f32_bits; int64 elem_type } */
@@ -216,9 +219,10 @@ uint32_t afir_hip_launch_norm_gate_residual(uint32_t block_dim, void *stream, vo
  * packed).  dy NULL: zero.  dh NULL (then also y, pre_weight, dpre_weight): the
  * call had no h.  f NULL (then also post_weight, gate and their gradients and
  * df): it had no f.  dx may be dy and df may be f; dx and df must not overlap,
- * as y and h above.  workspace: a device buffer
- * of afir_hip_norm_gate_residual_backward_workspace_bytes(tiling) bytes, one
- * for each of the launches that may overlap.
+ * as y and h above.  M = 0 is refused: nothing would write the weights'
+ * gradients.  workspace: a device buffer of
+ * afir_hip_norm_gate_residual_backward_workspace_bytes(tiling) bytes, one for
+ * each of the launches that may overlap.
  * TilingData { int64 dim_arg0_0 (M); int64 dim_arg0_1 (N); int64 rows_per_gate;
  *              int64 ld_dy, ld_dh, ld_y, ld_f, ld_gate, ld_dx, ld_df;
  *              int64 residual_scale_f32_bits; int64 eps_f32_bits; int64 elem_type } */
